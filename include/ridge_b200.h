@@ -239,6 +239,85 @@ int ridge_gemm_launch_variant(int index, const void* A, const void* B, void* C, 
  */
 int ridge_device_error(int clear, int32_t* code);
 
+/* ---------------------------------------------------------------- 8-bit operands */
+
+/*
+ * Operators of a linear layer with 8-bit operands (no counterpart in the
+ * reference): three that quantise rows -- plain, behind an RMS norm with the
+ * residual's addition, behind a gated activation --, the way back, and the
+ * product that reads what they write. An 8-bit array is rows of signed bytes
+ * in -127..127 with one FP32 scale per row; it stands for scale[i] * q[i][j].
+ *
+ * Element types of the arrays that are not 8-bit.
+ */
+enum { RIDGE_F16 = 0, RIDGE_BF16 = 1, RIDGE_F32 = 2 };
+
+/*
+ * Quantises the M rows of x (D elements each, pitch ldx elements) to
+ * q (pitch ldq bytes) and scale (M floats, contiguous):
+ *   scale[i] = max_j |x[i][j]| / 127,   q[i][j] = x[i][j] / scale[i] to the
+ * nearest whole number, ties to even (computed in FP32 with one rounded
+ * reciprocal, so an element within 2^-23 relative of a tie may go either way).
+ * A row of zeros has scale 0 and q 0. A row with an infinity or a NaN has an
+ * infinite or NaN scale and q 0, so that its products are NaN. Rows need no
+ * alignment beyond their elements'; rows whose starts and lengths are multiples
+ * of 16 bytes are read fastest. No output may share bytes with an input or with
+ * another output (RIDGE_EINVAL). M and D may be 0. M, D < 2^31. A pitch is at
+ * least D, and ignored when there is one row. Asynchronous on `stream`; needs no
+ * workspace and can be captured into a graph.
+ */
+int ridge_quantize_i8(const void* x, int32_t type, int8_t* q, float* scale, int64_t M, int64_t D,
+                      int64_t ldx, int64_t ldq, void* stream);
+
+/*
+ * RMS norm of rows, with an addition in front of it and an 8-bit output:
+ *   h = x + residual              (residual and residual_out both given)
+ *     = x                         (both NULL)
+ *   y[j] = weight[j] * h[j] / sqrt(mean(h^2) + eps)
+ * residual_out receives h, rounded once to `type`; the norm reads the FP32 sum.
+ * q and scale are those of y, as ridge_quantize_i8 defines them. x, residual,
+ * residual_out and weight (D elements) are of `type`. residual_out may be x or
+ * residual itself (same pointer and pitch); otherwise outputs overlap nothing.
+ * eps is finite and > 0. The sum of squares is FP32: a row whose h^2 overflows it
+ * (|h| beyond about 1e19) normalises to zeros, as if its mean square were infinite.
+ */
+int ridge_rms_norm_i8(const void* x, const void* residual, const void* weight, int32_t type,
+                      void* residual_out, int8_t* q, float* scale, int64_t M, int64_t D,
+                      int64_t ldx, int64_t ldr, int64_t ldro, int64_t ldq, float eps,
+                      void* stream);
+
+/*
+ * Gated activation with an 8-bit output: y = up * gate / (1 + exp(-gate)), then
+ * as ridge_quantize_i8. gate and up are of `type`; they may be column windows of
+ * one wider array.
+ */
+int ridge_silu_mul_i8(const void* gate, const void* up, int32_t type, int8_t* q, float* scale,
+                      int64_t M, int64_t D, int64_t ldg, int64_t ldu, int64_t ldq, void* stream);
+
+/* out[i][j] = scale[i] * q[i][j], rounded once to `type`. */
+int ridge_dequantize_i8(const int8_t* q, const float* scale, int32_t type, void* out, int64_t M,
+                        int64_t D, int64_t ldq, int64_t ldo, void* stream);
+
+/*
+ * C[i][j] = scale_a[i] * scale_b[j] * sum_k A[i][k] * B[j][k]  (+ bias[j])
+ *   A        M x K signed 8-bit, pitch lda bytes; scale_a M floats (token scales)
+ *   B        N x K signed 8-bit, pitch ldb bytes; scale_b N floats (channel scales)
+ *   bias     N elements of `type`, or NULL
+ *   C        M x N of `type`, pitch ldc elements (>= N)
+ * The sum is a 32-bit integer, exact for every K < 2^17 (longer K is refused with
+ * RIDGE_EINVAL); it is rounded to FP32, scaled there, and rounded once more to
+ * `type`. A and B start on 16 bytes and lda, ldb are multiples of 16 (TMA); a
+ * pitch is ignored where there is one row. C needs only its elements' alignment, and pitch and bytes past column N are
+ * not touched. K may be 0 (C is then the bias, or 0). C overlaps no input. The
+ * tile is chosen from M, N, K and the device; results do not depend on it.
+ * Asynchronous on `stream`; needs no workspace and can be captured into a graph.
+ * Kernels use the bounded waits and the error word of the other launches
+ * (ridge_device_error).
+ */
+int ridge_gemm_i8(const int8_t* A, const float* scale_a, const int8_t* B, const float* scale_b,
+                  const void* bias, int32_t type, void* C, int64_t M, int64_t N, int64_t K,
+                  int64_t lda, int64_t ldb, int64_t ldc, void* stream);
+
 /* ---------------------------------------------------------------- synthetic inputs */
 
 /*

@@ -22,6 +22,11 @@ RIDGE_ERANGE = -5
 RIDGE_ENOSCRATCH = -6
 RIDGE_ECOMM = -7
 
+# Element types of the 8-bit operators' other arrays.
+RIDGE_F16 = 0
+RIDGE_BF16 = 1
+RIDGE_F32 = 2
+
 BOTTLENECKS = ["TENSOR_CORE", "SMEM", "HBM", "OCC", "WAVES", "ENVELOPE", "DOES_NOT_FIT",
                "EPILOGUE", "L2"]
 
@@ -129,6 +134,14 @@ SIGNATURES = {
     "ridge_gemm_launch_variant": (C.c_int, [C.c_int, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
                                             _i64, _i64, _vp]),
     "ridge_device_error": (C.c_int, [C.c_int, C.POINTER(_i32)]),
+    "ridge_quantize_i8": (C.c_int, [_vp, _i32, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
+    "ridge_rms_norm_i8": (C.c_int, [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+                                    _i64, _i64, C.c_float, _vp]),
+    "ridge_silu_mul_i8": (C.c_int, [_vp, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+                                    _vp]),
+    "ridge_dequantize_i8": (C.c_int, [_vp, _vp, _i32, _vp, _i64, _i64, _i64, _i64, _vp]),
+    "ridge_gemm_i8": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _i64,
+                                _i64, _i64, _vp]),
     "ridge_fill_lcg": (C.c_int, [_vp, _i64, C.POINTER(C.c_uint32), _i32, _vp]),
     "ridge_bottleneck_string": (C.c_char_p, [_i32]),
     "ridge_hw_b200": (C.c_int, [C.POINTER(HwC)]),

@@ -21,6 +21,7 @@
 #include <vector>
 
 #include "../../include/ridge_b200.h"
+#include "device_info.h"
 #include "gemm_registry.h"
 #include "gemm_sm100.cuh"
 
@@ -564,6 +565,18 @@ int fill_library_counters(int byte) {
 }
 
 }  // namespace
+
+int device_info(DeviceInfo* out) {
+    int st = RIDGE_OK;
+    DeviceState* dev = device_state(&st);
+    if (!dev) return st;
+    out->num_sms = dev->num_sms;
+    out->err_word = dev->err_word;
+    return int(cudaGetDevice(&out->device));
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encode_fn() { return tensor_map_encoder(); }
+
 }  // namespace ridge_b200
 
 using namespace ridge_b200;

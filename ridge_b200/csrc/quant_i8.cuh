@@ -1,0 +1,343 @@
+// Row operators that write 8-bit GEMM operands: each row of y becomes signed
+// 8-bit values q in -127..127 and one FP32 scale, y ~ scale * q, with
+//
+//   scale = max_j |y_j| / 127,   q_j = round_to_even(y_j / scale).
+//
+//   kQuant    y = x
+//   kNorm     y = w h / sqrt(mean(h^2) + eps),  h = x
+//   kNormAdd  the same with h = x + r, h also stored (rounded once, to the type of x;
+//             the norm reads the FP32 sum, not the rounded one)
+//   kSiluMul  y = x r / (1 + exp(-x))          (r is the up projection)
+//
+// One pass over the data: a row sits in the registers of the threads that read
+// it. The norm needs two sums over a row, of h^2 and the maximum of |y|, but
+// its factor 1 / sqrt(mean + eps) is the same for the whole row, so with
+// v = w h both are taken in one reduction:
+//
+//   scale = max|v| rstd / 127,   q_j = round(v_j * (127 / max|v|)),
+//
+// and rstd never touches the elements. The other operators have v = y, rstd = 1.
+//
+// Numerics: everything between load and store is FP32. q_j is v_j * inv + 1.5 * 2^23
+// in one fused multiply-add: the sum's unit is 1, so the add rounds the exact
+// product to the nearest whole number (ties to even) and the low byte of its
+// bits is q_j. inv = 127 / max|v| is rounded once, so a v_j within 2^-24 relative
+// of a rounding border may go to the other side; |q_j| <= 127 always. Rows whose
+// maximum is below 2^-100 are first scaled by 2^64 so that inv cannot overflow.
+// A row of zeros has scale 0. A row holding an infinity or a NaN has an
+// infinite or NaN scale and q = 0, so that whatever is computed from it is NaN
+// and other rows are untouched.
+
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace ridge_b200 {
+
+enum RowOp { kQuant = 0, kNorm = 1, kNormAdd = 2, kSiluMul = 3 };
+
+struct RowParams {
+    const void* x;
+    const void* r;  // kNormAdd: residual; kSiluMul: up projection
+    const void* w;  // kNorm, kNormAdd: gain
+    void* h;        // kNormAdd: x + r
+    int8_t* q;
+    float* scale;
+    int64_t ldx, ldr, ldh, ldq;  // row pitches in elements
+    int M, D;
+    float eps;
+};
+
+// Elements of one 16-byte load.
+template <typename T>
+constexpr int kVecOf = 16 / int(sizeof(T));
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+
+// VEC elements as they lie in memory: one 16-byte load, or a single element
+// where the row's start or length is no multiple of 16 bytes.
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Chunk {
+    T e[VEC];
+};
+
+template <int VEC>
+struct alignas(VEC) Bytes {
+    int8_t b[VEC];
+};
+
+// Low bytes of the rounded sums v * inv + 1.5 * 2^23, four to a word.
+__device__ __forceinline__ uint32_t round_bits(float v, float inv) {
+    return __float_as_uint(fmaf(v, inv, 12582912.0f));
+}
+
+template <int VEC>
+__device__ __forceinline__ void store_q(int8_t* dst, const float (&v)[VEC], float pre, float inv,
+                                        bool zero) {
+    if constexpr (VEC == 1) {
+        const uint32_t b = round_bits(v[0] * pre, inv);
+        *dst = zero ? int8_t(0) : int8_t(b & 0xffu);
+    } else {
+        uint32_t word[VEC / 4];
+#pragma unroll
+        for (int i = 0; i < VEC / 4; ++i) {
+            const uint32_t lo = __byte_perm(round_bits(v[4 * i] * pre, inv),
+                                            round_bits(v[4 * i + 1] * pre, inv), 0x0040);
+            const uint32_t hi = __byte_perm(round_bits(v[4 * i + 2] * pre, inv),
+                                            round_bits(v[4 * i + 3] * pre, inv), 0x0040);
+            word[i] = zero ? 0u : __byte_perm(lo, hi, 0x5410);
+        }
+        if constexpr (VEC == 8)
+            *reinterpret_cast<uint2*>(dst) = make_uint2(word[0], word[1]);
+        else
+            *reinterpret_cast<uint32_t*>(dst) = word[0];
+    }
+}
+
+// v and, for kNormAdd, the stored sum of one chunk; adds to the row's sum of
+// squares and raises the row's maximum of |v|. The maximum is kept on the bits
+// of |v|, whose order as unsigned numbers is that of the values with every NaN
+// above infinity, so a NaN is never dropped.
+template <typename T, int OP, int VEC>
+__device__ __forceinline__ void take_chunk(const Chunk<T, VEC>& x, const Chunk<T, VEC>& r,
+                                           const Chunk<T, VEC>& w, Chunk<T, VEC>& h,
+                                           float (&v)[VEC], float& sumsq, uint32_t& top) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        float a = to_f32(x.e[i]);
+        if constexpr (OP == kNormAdd) {
+            a += to_f32(r.e[i]);
+            h.e[i] = from_f32<T>(a);
+        }
+        if constexpr (OP == kNorm || OP == kNormAdd) {
+            sumsq = fmaf(a, a, sumsq);
+            a *= to_f32(w.e[i]);
+        }
+        if constexpr (OP == kSiluMul) {
+            // __expf is off by 2^-22 + |x| 2^-24 relative; for x > 0 that reaches y
+            // times e^-x, and for x << 0 y itself is small beside the row's maximum.
+            a = __fdividef(a, 1.0f + __expf(-a)) * to_f32(r.e[i]);
+        }
+        v[i] = a;
+        top = max(top, __float_as_uint(a) & 0x7fffffffu);
+    }
+}
+
+// What a row's two reductions make of its elements.
+struct RowScale {
+    float scale, pre, inv;
+    bool zero;
+};
+
+template <int OP>
+__device__ __forceinline__ RowScale row_scale(float sumsq, uint32_t top, int D, float eps) {
+    const float amax = __uint_as_float(top);
+    float rstd = 1.0f;
+    if constexpr (OP == kNorm || OP == kNormAdd) rstd = 1.0f / sqrtf(sumsq / float(D) + eps);
+    RowScale s;
+    s.scale = top == 0 ? 0.0f : amax * rstd / 127.0f;
+    s.zero = !(s.scale > 0.0f && s.scale < __uint_as_float(0x7f800000u));
+    s.pre = amax < 7.8886091e-31f ? 18446744073709551616.0f : 1.0f;  // 2^-100, 2^64
+    s.inv = 127.0f / (amax * s.pre);
+    return s;
+}
+
+// Sum and maximum over the G warps of a row (one warp: shuffles alone). Every
+// thread gets both; the order of the sum is fixed.
+__device__ __forceinline__ void reduce_row(float& sumsq, uint32_t& top, bool with_sum) {
+    __shared__ float s_sum[32];
+    __shared__ uint32_t s_top[32];
+    if (with_sum) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sumsq += __shfl_xor_sync(0xffffffffu, sumsq, o);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    const int G = blockDim.x >> 5;
+    if (G == 1) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) {
+        s_sum[warp] = sumsq;
+        s_top[warp] = top;
+    }
+    __syncthreads();
+    top = __reduce_max_sync(0xffffffffu, lane < G ? s_top[lane] : 0u);
+    if (with_sum) {
+        sumsq = lane < G ? s_sum[lane] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sumsq += __shfl_xor_sync(0xffffffffu, sumsq, o);
+    }
+}
+
+// One row per blockDim.x threads (a multiple of 32), blockDim.y rows per CTA
+// (more than one only for single-warp rows, which need no barrier). CH chunks
+// of VEC elements per thread.
+template <typename T, int OP, int VEC, int CH, int MAXT>
+__global__ void __launch_bounds__(MAXT) ridge_row_i8(const RowParams p) {
+    constexpr bool kR = OP == kNormAdd || OP == kSiluMul;
+    constexpr bool kW = OP == kNorm || OP == kNormAdd;
+    const int64_t row = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
+    if (row >= p.M) return;
+    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+    const T* r = static_cast<const T*>(p.r) + (kR ? row * p.ldr : 0);
+    const T* w = static_cast<const T*>(p.w);
+    using C = Chunk<T, VEC>;
+    C cx[CH], cr[kR ? CH : 1], cw[kW ? CH : 1];
+    // Every load of the row is issued before the first value is used.
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int e = (c * int(blockDim.x) + int(threadIdx.x)) * VEC;
+        if (e < p.D) {
+            cx[c] = *reinterpret_cast<const C*>(x + e);
+            if constexpr (kR) cr[c] = *reinterpret_cast<const C*>(r + e);
+            if constexpr (kW) cw[c] = *reinterpret_cast<const C*>(w + e);
+        }
+    }
+    float v[CH][VEC];
+    float sumsq = 0.0f;
+    uint32_t top = 0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int e = (c * int(blockDim.x) + int(threadIdx.x)) * VEC;
+        if (e < p.D) {
+            C h;
+            take_chunk<T, OP, VEC>(cx[c], cr[kR ? c : 0], cw[kW ? c : 0], h, v[c], sumsq, top);
+            if constexpr (OP == kNormAdd)
+                *reinterpret_cast<C*>(static_cast<T*>(p.h) + row * p.ldh + e) = h;
+        }
+    }
+    reduce_row(sumsq, top, kW);
+    const RowScale s = row_scale<OP>(sumsq, top, p.D, p.eps);
+    int8_t* q = p.q + row * p.ldq;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int e = (c * int(blockDim.x) + int(threadIdx.x)) * VEC;
+        if (e < p.D) store_q<VEC>(q + e, v[c], s.pre, s.inv, s.zero);
+    }
+    if (threadIdx.x == 0) p.scale[row] = s.scale;
+}
+
+// Rows longer than a CTA's registers hold: read twice (the second time mostly
+// from L2), reduce in the first pass and write in the second. x + r is stored
+// in the second pass only, each element by the thread that has just read it,
+// so h may be x or r here too.
+template <typename T, int OP, int VEC>
+__global__ void __launch_bounds__(1024) ridge_row_i8_long(const RowParams p) {
+    constexpr bool kR = OP == kNormAdd || OP == kSiluMul;
+    constexpr bool kW = OP == kNorm || OP == kNormAdd;
+    const int64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+    const T* r = static_cast<const T*>(p.r) + (kR ? row * p.ldr : 0);
+    const T* w = static_cast<const T*>(p.w);
+    using C = Chunk<T, VEC>;
+    const int64_t step = int64_t(blockDim.x) * VEC;
+    float sumsq = 0.0f;
+    uint32_t top = 0;
+    C cx, cr, cw, h;
+    float v[VEC];
+    auto load = [&](int64_t e) {
+        cx = *reinterpret_cast<const C*>(x + e);
+        if constexpr (kR) cr = *reinterpret_cast<const C*>(r + e);
+        if constexpr (kW) cw = *reinterpret_cast<const C*>(w + e);
+    };
+    for (int64_t e = int64_t(threadIdx.x) * VEC; e < p.D; e += step) {
+        load(e);
+        take_chunk<T, OP, VEC>(cx, cr, cw, h, v, sumsq, top);
+    }
+    reduce_row(sumsq, top, kW);
+    const RowScale s = row_scale<OP>(sumsq, top, p.D, p.eps);
+    int8_t* q = p.q + row * p.ldq;
+    float unused_sum = 0.0f;
+    uint32_t unused_top = 0;
+    for (int64_t e = int64_t(threadIdx.x) * VEC; e < p.D; e += step) {
+        load(e);
+        take_chunk<T, OP, VEC>(cx, cr, cw, h, v, unused_sum, unused_top);
+        if constexpr (OP == kNormAdd)
+            *reinterpret_cast<C*>(static_cast<T*>(p.h) + row * p.ldh + e) = h;
+        store_q<VEC>(q + e, v, s.pre, s.inv, s.zero);
+    }
+    if (threadIdx.x == 0) p.scale[row] = s.scale;
+}
+
+template <typename T, int OP, int VEC, int CH, int MAXT>
+cudaError_t launch_rows(const RowParams& p, int threads, int rows_per_cta, cudaStream_t stream) {
+    const dim3 block(static_cast<unsigned>(threads), static_cast<unsigned>(rows_per_cta));
+    const unsigned grid = unsigned((int64_t(p.M) + rows_per_cta - 1) / rows_per_cta);
+    ridge_row_i8<T, OP, VEC, CH, MAXT><<<grid, block, 0, stream>>>(p);
+    return cudaGetLastError();
+}
+
+// The launch shape of a row of `chunks` loads. Rows of up to 128 loads take one
+// warp, four rows to a CTA (no barrier). Longer rows take a CTA with as few
+// chunks per thread as fit when there are fewer rows than SMs -- one row's
+// latency is then all that counts -- and four per thread otherwise, so that
+// several CTAs share an SM and one row's reduction hides behind another's loads.
+template <typename T, int OP, int VEC>
+cudaError_t run_rows(const RowParams& p, int num_sms, cudaStream_t stream) {
+    const int64_t chunks = (int64_t(p.D) + VEC - 1) / VEC;
+    auto threads_for = [&](int per) { return int(((chunks + per - 1) / per + 31) / 32 * 32); };
+    if constexpr (VEC > 1) {
+        if (chunks <= 32) return launch_rows<T, OP, VEC, 1, 1024>(p, 32, 4, stream);
+        if (chunks <= 64) return launch_rows<T, OP, VEC, 2, 1024>(p, 32, 4, stream);
+        if (chunks <= 128) return launch_rows<T, OP, VEC, 4, 512>(p, 32, 4, stream);
+        if (p.M <= num_sms) {
+            if (chunks <= 1024) return launch_rows<T, OP, VEC, 1, 1024>(p, threads_for(1), 1, stream);
+            if (chunks <= 2048) return launch_rows<T, OP, VEC, 2, 1024>(p, threads_for(2), 1, stream);
+        }
+        if (chunks <= 2048) return launch_rows<T, OP, VEC, 4, 512>(p, threads_for(4), 1, stream);
+        if (chunks <= 4096) return launch_rows<T, OP, VEC, 4, 1024>(p, threads_for(4), 1, stream);
+    } else {
+        if (chunks <= 128) return launch_rows<T, OP, VEC, 4, 1024>(p, 32, 4, stream);
+        if (chunks <= 4096) return launch_rows<T, OP, VEC, 4, 1024>(p, threads_for(4), 1, stream);
+        if (chunks <= 16384) return launch_rows<T, OP, VEC, 16, 1024>(p, threads_for(16), 1, stream);
+    }
+    ridge_row_i8_long<T, OP, VEC><<<unsigned(p.M), 1024, 0, stream>>>(p);
+    return cudaGetLastError();
+}
+
+// 16-byte loads need every row of every operand to start on 16 bytes and D to be
+// whole chunks; q then takes 8- or 4-byte stores.
+template <typename T, int OP>
+cudaError_t run_op(const RowParams& p, int num_sms, cudaStream_t stream) {
+    constexpr int V = kVecOf<T>;
+    auto fits = [](const void* ptr, int64_t ld, int size, int bytes) {
+        return (reinterpret_cast<uintptr_t>(ptr) % bytes) == 0 && (ld * size) % bytes == 0;
+    };
+    bool vec = p.D % V == 0 && fits(p.x, p.ldx, sizeof(T), 16) && fits(p.q, p.ldq, 1, V);
+    if (OP == kNormAdd || OP == kSiluMul) vec = vec && fits(p.r, p.ldr, sizeof(T), 16);
+    if (OP == kNorm || OP == kNormAdd) vec = vec && fits(p.w, 0, 1, 16);
+    if (OP == kNormAdd) vec = vec && fits(p.h, p.ldh, sizeof(T), 16);
+    return vec ? run_rows<T, OP, V>(p, num_sms, stream) : run_rows<T, OP, 1>(p, num_sms, stream);
+}
+
+template <typename T>
+cudaError_t run_type(int op, const RowParams& p, int num_sms, cudaStream_t stream) {
+    switch (op) {
+        case kQuant: return run_op<T, kQuant>(p, num_sms, stream);
+        case kNorm: return run_op<T, kNorm>(p, num_sms, stream);
+        case kNormAdd: return run_op<T, kNormAdd>(p, num_sms, stream);
+        default: return run_op<T, kSiluMul>(p, num_sms, stream);
+    }
+}
+
+// One translation unit per element type (quant_i8_*.cu).
+cudaError_t run_rows_f16(int op, const RowParams& p, int num_sms, cudaStream_t stream);
+cudaError_t run_rows_bf16(int op, const RowParams& p, int num_sms, cudaStream_t stream);
+cudaError_t run_rows_f32(int op, const RowParams& p, int num_sms, cudaStream_t stream);
+
+}  // namespace ridge_b200

@@ -1,0 +1,10 @@
+// The BF16 instances of the row operators (quant_i8.cuh).
+#include "quant_i8.cuh"
+
+namespace ridge_b200 {
+
+cudaError_t run_rows_bf16(int op, const RowParams& p, int num_sms, cudaStream_t stream) {
+    return run_type<__nv_bfloat16>(op, p, num_sms, stream);
+}
+
+}  // namespace ridge_b200

@@ -1,0 +1,194 @@
+// C-ABI front end of the row operators (quant_i8.cuh) and the kernel that turns
+// 8-bit rows and their scales back into values (include/ridge_b200.h).
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/ridge_b200.h"
+#include "device_info.h"
+#include "quant_i8.cuh"
+#include "row_arrays.h"
+
+namespace ridge_b200 {
+namespace {
+
+bool extents_ok(int64_t M, int64_t D) {
+    return M >= 0 && D >= 0 && M < (int64_t(1) << 31) && D < (int64_t(1) << 31);
+}
+
+int run(int op, int32_t type, RowParams p, int64_t M, int64_t D, void* stream_v) {
+    const int size = type_size(type);
+    if (size == 0 || !extents_ok(M, D)) return RIDGE_EINVAL;
+    const bool has_r = op == kNormAdd || op == kSiluMul;
+    const bool has_w = op == kNorm || op == kNormAdd;
+    if (M == 0) return RIDGE_OK;
+    if (!array_ok(p.x, M, D, p.ldx, size) || !array_ok(p.q, M, D, p.ldq, 1) ||
+        !array_ok(p.scale, M, 1, 1, 4))
+        return RIDGE_EINVAL;
+    if (has_r && !array_ok(p.r, M, D, p.ldr, size)) return RIDGE_EINVAL;
+    if (has_w && !array_ok(p.w, 1, D, D, size)) return RIDGE_EINVAL;
+    if (op == kNormAdd && !array_ok(p.h, M, D, p.ldh, size)) return RIDGE_EINVAL;
+    if (M == 1) p.ldx = p.ldr = p.ldh = p.ldq = D;
+    // Outputs against inputs and against one another. h may be x or r itself.
+    const RowArray in[3] = {{p.x, M, p.ldx * size, D * size},
+                            {has_r ? p.r : nullptr, M, p.ldr * size, D * size},
+                            {has_w ? p.w : nullptr, 1, D * size, D * size}};
+    const RowArray q = {p.q, M, p.ldq, D}, sc = {p.scale, 1, M * 4, M * 4};
+    const RowArray h = {op == kNormAdd ? p.h : nullptr, M, p.ldh * size, D * size};
+    for (const RowArray& a : in) {
+        if (overlaps(q, a) || overlaps(sc, a)) return RIDGE_EINVAL;
+        if (overlaps(h, a) && !(a.p == h.p && a.pitch == h.pitch && a.rows == h.rows))
+            return RIDGE_EINVAL;
+    }
+    if (overlaps(q, h) || overlaps(sc, h) || overlaps(q, sc)) return RIDGE_EINVAL;
+    DeviceInfo dev;
+    const int st = device_info(&dev);
+    if (st != RIDGE_OK) return st;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+    if (D == 0) return int(cudaMemsetAsync(p.scale, 0, size_t(M) * 4, stream));
+    p.M = int(M);
+    p.D = int(D);
+    cudaError_t e;
+    if (type == RIDGE_F16) e = run_rows_f16(op, p, dev.num_sms, stream);
+    else if (type == RIDGE_BF16) e = run_rows_bf16(op, p, dev.num_sms, stream);
+    else e = run_rows_f32(op, p, dev.num_sms, stream);
+    return int(e);
+}
+
+// Values of 8-bit rows: out = scale[row] * q, one rounding to T. A thread takes
+// 16 values (one 16-byte load, 32 or 64 bytes of stores) at a time; blockDim.x
+// threads walk a row and blockDim.y rows share a CTA, so short rows fill one.
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(256)
+    ridge_dequantize_i8(const int8_t* __restrict__ q, const float* __restrict__ scale,
+                        T* __restrict__ out, int M, int D, int64_t ldq, int64_t ldo) {
+    const int64_t row = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
+    if (row >= M) return;
+    const float s = scale[row];
+    const int8_t* src = q + row * ldq;
+    T* dst = out + row * ldo;
+    constexpr int kPer = kVec ? 16 : 1;
+    const int64_t first = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * kPer;
+    const int64_t step = int64_t(gridDim.y) * blockDim.x * kPer;
+    for (int64_t e = first; e < D; e += step) {
+        if constexpr (kVec) {
+            const Chunk<int8_t, 16> in = *reinterpret_cast<const Chunk<int8_t, 16>*>(src + e);
+            constexpr int V = kVecOf<T>;
+#pragma unroll
+            for (int g = 0; g < 16 / V; ++g) {
+                Chunk<T, V> o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o.e[i] = from_f32<T>(float(in.e[g * V + i]) * s);
+                *reinterpret_cast<Chunk<T, V>*>(dst + e + g * V) = o;
+            }
+        } else {
+            dst[e] = from_f32<T>(float(src[e]) * s);
+        }
+    }
+}
+
+template <typename T>
+cudaError_t run_dequantize(const int8_t* q, const float* scale, void* out_v, int M, int D,
+                           int64_t ldq, int64_t ldo, int num_sms, cudaStream_t stream) {
+    T* out = static_cast<T*>(out_v);
+    const bool vec = D % 16 == 0 && ldq % 16 == 0 && (ldo * int64_t(sizeof(T))) % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(out) % 16 == 0;
+    const int64_t per_row = vec ? D / 16 : D;
+    int tx = 32;
+    while (tx < 256 && tx < per_row) tx *= 2;
+    const int ty = 256 / tx;
+    const int64_t row_ctas = (int64_t(M) + ty - 1) / ty;
+    // With fewer rows than would fill the GPU a row is split over several CTAs.
+    const int64_t want = std::max<int64_t>(1, int64_t(num_sms) * 8 / row_ctas);
+    const int64_t most = (per_row + tx - 1) / tx;
+    const dim3 grid(unsigned(row_ctas), unsigned(std::min<int64_t>({want, most, 65535})));
+    const dim3 block(static_cast<unsigned>(tx), static_cast<unsigned>(ty));
+    if (vec)
+        ridge_dequantize_i8<T, true><<<grid, block, 0, stream>>>(q, scale, out, M, D, ldq, ldo);
+    else
+        ridge_dequantize_i8<T, false><<<grid, block, 0, stream>>>(q, scale, out, M, D, ldq, ldo);
+    return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace ridge_b200
+
+using namespace ridge_b200;
+
+extern "C" {
+
+int ridge_quantize_i8(const void* x, int32_t type, int8_t* q, float* scale, int64_t M, int64_t D,
+                      int64_t ldx, int64_t ldq, void* stream) {
+    RowParams p{};
+    p.x = x;
+    p.q = q;
+    p.scale = scale;
+    p.ldx = ldx;
+    p.ldq = ldq;
+    return run(kQuant, type, p, M, D, stream);
+}
+
+int ridge_rms_norm_i8(const void* x, const void* residual, const void* weight, int32_t type,
+                      void* residual_out, int8_t* q, float* scale, int64_t M, int64_t D,
+                      int64_t ldx, int64_t ldr, int64_t ldro, int64_t ldq, float eps,
+                      void* stream) {
+    if (!(eps > 0.0f) || !std::isfinite(eps)) return RIDGE_EINVAL;
+    if ((residual == nullptr) != (residual_out == nullptr) && M > 0 && D > 0) return RIDGE_EINVAL;
+    RowParams p{};
+    p.x = x;
+    p.r = residual;
+    p.w = weight;
+    p.h = residual_out;
+    p.q = q;
+    p.scale = scale;
+    p.ldx = ldx;
+    p.ldr = ldr;
+    p.ldh = ldro;
+    p.ldq = ldq;
+    p.eps = eps;
+    return run(residual ? kNormAdd : kNorm, type, p, M, D, stream);
+}
+
+int ridge_silu_mul_i8(const void* gate, const void* up, int32_t type, int8_t* q, float* scale,
+                      int64_t M, int64_t D, int64_t ldg, int64_t ldu, int64_t ldq, void* stream) {
+    RowParams p{};
+    p.x = gate;
+    p.r = up;
+    p.q = q;
+    p.scale = scale;
+    p.ldx = ldg;
+    p.ldr = ldu;
+    p.ldq = ldq;
+    return run(kSiluMul, type, p, M, D, stream);
+}
+
+int ridge_dequantize_i8(const int8_t* q, const float* scale, int32_t type, void* out, int64_t M,
+                        int64_t D, int64_t ldq, int64_t ldo, void* stream_v) {
+    const int size = type_size(type);
+    if (size == 0 || !extents_ok(M, D)) return RIDGE_EINVAL;
+    if (M == 0 || D == 0) return RIDGE_OK;
+    if (!array_ok(q, M, D, ldq, 1) || !array_ok(scale, M, 1, 1, 4) ||
+        !array_ok(out, M, D, ldo, size))
+        return RIDGE_EINVAL;
+    if (M == 1) ldq = ldo = D;
+    const RowArray o = {out, M, ldo * size, D * size};
+    if (overlaps(o, {q, M, ldq, D}) || overlaps(o, {scale, 1, M * 4, M * 4})) return RIDGE_EINVAL;
+    DeviceInfo dev;
+    const int st = device_info(&dev);
+    if (st != RIDGE_OK) return st;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+    cudaError_t e;
+    if (type == RIDGE_F16)
+        e = run_dequantize<__half>(q, scale, out, int(M), int(D), ldq, ldo, dev.num_sms, stream);
+    else if (type == RIDGE_BF16)
+        e = run_dequantize<__nv_bfloat16>(q, scale, out, int(M), int(D), ldq, ldo, dev.num_sms,
+                                          stream);
+    else
+        e = run_dequantize<float>(q, scale, out, int(M), int(D), ldq, ldo, dev.num_sms, stream);
+    return int(e);
+}
+
+}  // extern "C"

@@ -1,0 +1,254 @@
+"""Linear layers with 8-bit operands: quantising rows (plain, behind an RMS norm,
+behind a gated activation), the way back, and the int8 GEMM that reads them.
+
+An 8-bit array is a pair (q, scale): q (M, D) int8 in -127..127 and scale (M,)
+float32, standing for scale[i] * q[i, j]. Activations are quantised by token and
+weights by output channel, both with the rows contiguous, so
+
+    q, s, h = rms_norm_i8(x, gain, residual=h)          # h += x; q ~ gain * h / rms(h)
+    y = gemm_i8(q, s, w_q, w_scale)                     # w_q, w_scale = quantize_i8(w)
+
+is a linear layer with w (N, K) behind a norm. The C ABI is in
+include/ridge_b200.h; like `gemm`, the calls launch on `stream` (default: torch's
+current stream of the tensors' device) and never synchronise. They check what can
+be checked on the host and raise TypeError, ValueError or RidgeError before
+anything is launched.
+
+Outputs that a call allocates come from the pool of the stream it launches on.
+q is allocated with its row pitch rounded up to 16 bytes, which is what gemm_i8
+needs; pass `out` to write into an array of your own.
+"""
+
+from __future__ import annotations
+
+import math
+
+from ._native import RIDGE_BF16, RIDGE_F16, RIDGE_F32, check, lib
+
+_TYPES = None
+
+
+def _type_code(dtype, what):
+    global _TYPES
+    if _TYPES is None:
+        import torch
+        _TYPES = {torch.float16: RIDGE_F16, torch.bfloat16: RIDGE_BF16, torch.float32: RIDGE_F32}
+    code = _TYPES.get(dtype)
+    if code is None:
+        raise TypeError("%s is float16, bfloat16 or float32, not %s" % (what, dtype))
+    return code
+
+
+def _rows(t, what):
+    """(M, D, pitch) of a 2-D CUDA tensor with contiguous rows."""
+    if t.dim() != 2:
+        raise ValueError("%s is a matrix of rows, got shape %s" % (what, tuple(t.shape)))
+    if not t.is_cuda:
+        raise ValueError("%s is not a CUDA tensor" % what)
+    M, D = t.shape
+    if D > 1 and t.stride(1) != 1:
+        raise ValueError("%s: rows must be contiguous (inner stride 1)" % what)
+    pitch = t.stride(0)
+    if M > 1:
+        if pitch < D:
+            raise ValueError("%s: rows overlap (pitch %d, length %d)" % (what, pitch, D))
+    elif pitch < D:
+        pitch = D
+    return M, D, pitch
+
+
+def _like(t, what, device, dtype, shape):
+    """Checks a tensor that has to match another in device, type and shape."""
+    if t.device != device:
+        raise ValueError("%s is on %s, expected %s" % (what, t.device, device))
+    if t.dtype != dtype:
+        raise TypeError("%s is %s, expected %s" % (what, t.dtype, dtype))
+    if t.shape != shape:
+        raise ValueError("%s has shape %s, expected %s" % (what, tuple(t.shape), tuple(shape)))
+
+
+def _vector(t, what, device, dtype, n):
+    _like(t, what, device, dtype, (n,))
+    if n > 1 and t.stride(0) != 1:
+        raise ValueError("%s must be contiguous" % what)
+
+
+class _Launch:
+    """The device and stream of one call: makes the tensors' device current and,
+    for a stream other than torch's current one, allocates from its pool."""
+
+    __slots__ = ("handle", "_contexts")
+
+    def __init__(self, device, stream):
+        import torch
+        index = device.index
+        self._contexts = ()
+        if index != torch.cuda.current_device():
+            self._contexts = (torch.cuda.device(index),)
+        if stream is None:
+            self.handle = torch._C._cuda_getCurrentRawStream(index)
+            return
+        self.handle = stream if isinstance(stream, int) else stream.cuda_stream
+        if self.handle != torch._C._cuda_getCurrentRawStream(index):
+            if self.handle == 0:
+                s = torch.cuda.default_stream(index)
+            elif isinstance(stream, int):
+                s = torch.cuda.ExternalStream(stream, device=index)
+            else:
+                s = stream
+            self._contexts += (torch.cuda.stream(s),)
+
+    def __enter__(self):
+        for c in self._contexts:
+            c.__enter__()
+        return self.handle
+
+    def __exit__(self, *exc):
+        for c in reversed(self._contexts):
+            c.__exit__(*exc)
+
+
+def _outputs(M, D, device, out, scale):
+    """(q, q's pitch, scale): the given arrays, checked, or new ones."""
+    import torch
+    if out is None:
+        pitch = (D + 15) // 16 * 16
+        out = torch.empty((M, pitch), dtype=torch.int8, device=device)
+        if pitch != D:
+            out = out[:, :D]
+    else:
+        _like(out, "out", device, torch.int8, (M, D))
+        pitch = _rows(out, "out")[2]
+    if scale is None:
+        scale = torch.empty(M, dtype=torch.float32, device=device)
+    else:
+        _vector(scale, "scale", device, torch.float32, M)
+    return out, pitch, scale
+
+
+def quantize_i8(x, out=None, scale=None, stream=None):
+    """(q, scale) of the rows of x (M, D), float16, bfloat16 or float32:
+    scale = max |row| / 127, q = row / scale to the nearest whole number. A row of
+    zeros has scale 0; a row with an infinity or NaN has a scale that is not
+    finite, and q = 0."""
+    code = _type_code(x.dtype, "x")
+    M, D, ldx = _rows(x, "x")
+    with _Launch(x.device, stream) as handle:
+        q, ldq, scale = _outputs(M, D, x.device, out, scale)
+        check(lib.ridge_quantize_i8(x.data_ptr(), code, q.data_ptr(), scale.data_ptr(), M, D, ldx,
+                                    ldq, handle), "ridge_quantize_i8 %dx%d" % (M, D))
+    return q, scale
+
+
+def rms_norm_i8(x, weight, residual=None, eps=1e-6, out=None, scale=None, residual_out=None,
+                stream=None):
+    """(q, scale, h) of y = weight * h / sqrt(mean(h^2) + eps) with h = x + residual,
+    or h = x without one (h is then returned as None).
+
+    x, residual (M, D) and weight (D,) have one type. h is rounded once to that type;
+    the norm reads the unrounded sum. residual_out receives h and may be residual
+    or x itself; by default it is a new tensor."""
+    import torch
+    code = _type_code(x.dtype, "x")
+    M, D, ldx = _rows(x, "x")
+    _vector(weight, "weight", x.device, x.dtype, D)
+    eps = float(eps)
+    if not (eps > 0 and math.isfinite(eps)):
+        raise ValueError("eps is finite and above 0, got %r" % eps)
+    if residual is None and residual_out is not None:
+        raise ValueError("residual_out needs a residual")
+    ldr = ldh = D
+    if residual is not None:
+        _like(residual, "residual", x.device, x.dtype, x.shape)
+        ldr = _rows(residual, "residual")[2]
+        if residual_out is not None:
+            _like(residual_out, "residual_out", x.device, x.dtype, x.shape)
+            ldh = _rows(residual_out, "residual_out")[2]
+    with _Launch(x.device, stream) as handle:
+        q, ldq, scale = _outputs(M, D, x.device, out, scale)
+        if residual is not None and residual_out is None:
+            residual_out = torch.empty((M, D), dtype=x.dtype, device=x.device)
+        # An empty tensor's address is null, which at the C ABI means "not given".
+        given = residual is not None and M > 0 and D > 0
+        check(lib.ridge_rms_norm_i8(x.data_ptr(), residual.data_ptr() if given else None,
+                                    weight.data_ptr(), code,
+                                    residual_out.data_ptr() if given else None, q.data_ptr(),
+                                    scale.data_ptr(), M, D, ldx, ldr, ldh, ldq, eps, handle),
+              "ridge_rms_norm_i8 %dx%d" % (M, D))
+    return q, scale, residual_out
+
+
+def silu_mul_i8(gate, up, out=None, scale=None, stream=None):
+    """(q, scale) of y = up * gate / (1 + exp(-gate)). gate and up (M, D) have one
+    type and may be the two halves of one (M, 2 D) tensor."""
+    code = _type_code(gate.dtype, "gate")
+    M, D, ldg = _rows(gate, "gate")
+    _like(up, "up", gate.device, gate.dtype, gate.shape)
+    ldu = _rows(up, "up")[2]
+    with _Launch(gate.device, stream) as handle:
+        q, ldq, scale = _outputs(M, D, gate.device, out, scale)
+        check(lib.ridge_silu_mul_i8(gate.data_ptr(), up.data_ptr(), code, q.data_ptr(),
+                                    scale.data_ptr(), M, D, ldg, ldu, ldq, handle),
+              "ridge_silu_mul_i8 %dx%d" % (M, D))
+    return q, scale
+
+
+def dequantize_i8(q, scale, out=None, dtype=None, stream=None):
+    """The values scale[i] * q[i, j], rounded once to dtype (float16 by default,
+    or that of `out`)."""
+    import torch
+    if q.dtype != torch.int8:
+        raise TypeError("q is int8, got %s" % q.dtype)
+    M, D, ldq = _rows(q, "q")
+    _vector(scale, "scale", q.device, torch.float32, M)
+    if dtype is None:
+        dtype = torch.float16 if out is None else out.dtype
+    code = _type_code(dtype, "dtype")
+    ldo = D
+    if out is not None:
+        _like(out, "out", q.device, dtype, q.shape)
+        ldo = _rows(out, "out")[2]
+    with _Launch(q.device, stream) as handle:
+        if out is None:
+            out = torch.empty((M, D), dtype=dtype, device=q.device)
+        check(lib.ridge_dequantize_i8(q.data_ptr(), scale.data_ptr(), code, out.data_ptr(), M, D,
+                                      ldq, ldo, handle), "ridge_dequantize_i8 %dx%d" % (M, D))
+    return out
+
+
+def gemm_i8(a, a_scale, b, b_scale, bias=None, out=None, dtype=None, stream=None):
+    """out[i, j] = a_scale[i] * b_scale[j] * sum_k a[i, k] * b[j, k] (+ bias[j]).
+
+    a (M, K) and b (N, K) int8 with float32 scales (M,) and (N,), as the quantising
+    calls return them; out (M, N) float16 (default), bfloat16 or float32, bias (N,)
+    of that type. The integer sum is exact (K < 131072). a and b start on 16 bytes
+    and their row pitches are multiples of 16 (RidgeError otherwise)."""
+    import torch
+    if a.dtype != torch.int8 or b.dtype != torch.int8:
+        raise TypeError("ridge_b200.gemm_i8 takes int8 operands")
+    M, K, lda = _rows(a, "a")
+    N, Kb, ldb = _rows(b, "b")
+    if K != Kb:
+        raise ValueError("expected a (M, K) and b (N, K), got %s and %s" % (tuple(a.shape),
+                                                                         tuple(b.shape)))
+    if b.device != a.device:
+        raise ValueError("b is on %s, expected %s" % (b.device, a.device))
+    _vector(a_scale, "a_scale", a.device, torch.float32, M)
+    _vector(b_scale, "b_scale", a.device, torch.float32, N)
+    if dtype is None:
+        dtype = torch.float16 if out is None else out.dtype
+    code = _type_code(dtype, "dtype")
+    if bias is not None:
+        _vector(bias, "bias", a.device, dtype, N)
+    ldc = N
+    if out is not None:
+        _like(out, "out", a.device, dtype, (M, N))
+        ldc = _rows(out, "out")[2]
+    with _Launch(a.device, stream) as handle:
+        if out is None:
+            out = torch.empty((M, N), dtype=dtype, device=a.device)
+        check(lib.ridge_gemm_i8(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(),
+                                b_scale.data_ptr(), None if bias is None else bias.data_ptr(),
+                                code, out.data_ptr(), M, N, K, lda, ldb, ldc, handle),
+              "ridge_gemm_i8 %dx%dx%d" % (M, N, K))
+    return out
