@@ -253,8 +253,7 @@ extern "C" int ridge_gemm_i8(const int8_t* A, const float* scale_a, const int8_t
     p.bn = plan.bn;
     p.stages = plan.stages;
     p.groupM = 8;
-    p.sb_vec = (reinterpret_cast<uintptr_t>(scale_b) & 15) == 0 &&
-               (reinterpret_cast<uintptr_t>(bias) & 15) == 0;
+    p.vec_store = reinterpret_cast<uintptr_t>(C) % uintptr_t(4 * size) == 0 && ldc % 4 == 0;
     // Stores through the tensor map need 16-byte aligned rows of C.
     p.tma_store = (reinterpret_cast<uintptr_t>(C) & 15) == 0 && (ldc * size) % 16 == 0;
     CUtensorMap tmap_a, tmap_b, tmap_c;

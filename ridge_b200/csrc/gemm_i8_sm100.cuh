@@ -55,7 +55,7 @@ struct I8Params {
     int stages;
     int groupM;
     int tma_store;  // tile: C is stored through its tensor map; 0: from shared memory by threads
-    int sb_vec;     // tile: sb and bias can be read four at a time
+    int vec_store;  // stream: rows of C start on four elements
     int* err;
 };
 
@@ -85,35 +85,25 @@ struct OutType<float> {
     __device__ static float down(float v) { return v; }
 };
 
-// Four consecutive values of a vector of n, from col on; zeros past its end.
-template <typename T>
-__device__ __forceinline__ float4 load_cols(const T* v, int col, int n, bool vec) {
-    if (vec && col + 4 <= n) {
-        if constexpr (sizeof(T) == 4) {
-            return __ldg(reinterpret_cast<const float4*>(v + col));
-        } else {
-            const uint2 u = __ldg(reinterpret_cast<const uint2*>(v + col));
-            const T* e = reinterpret_cast<const T*>(&u);
-            return make_float4(OutType<T>::up(e[0]), OutType<T>::up(e[1]), OutType<T>::up(e[2]),
-                               OutType<T>::up(e[3]));
-        }
-    }
-    return make_float4(col < n ? OutType<T>::up(v[col]) : 0.0f,
-                       col + 1 < n ? OutType<T>::up(v[col + 1]) : 0.0f,
-                       col + 2 < n ? OutType<T>::up(v[col + 2]) : 0.0f,
-                       col + 3 < n ? OutType<T>::up(v[col + 3]) : 0.0f);
-}
-
 // ------------------------------------------------------------------ tiles by 2-CTA pairs
 
 constexpr int kI8TileThreads = 10 * 32;  // producer, MMA, 8 epilogue warps
-constexpr int kI8TileEpiBytes = 8 * 4096;
+constexpr int kI8TileStageOut = 4096;  // 32 rows x 128 bytes of C per epilogue warp
+constexpr int kI8TileCols = 2 * 64;    // columns of a tile that one epilogue warp drains
+constexpr int kI8TileEpiBytes = 8 * (kI8TileStageOut + kI8TileCols * 8);
 
 __host__ __device__ constexpr int i8_tile_stage_bytes(int bn) {
     return 128 * kI8BK + (bn / 2) * kI8BK;
 }
 constexpr int i8_tile_smem(int bn, int stages) {
     return kI8AlignSlack + stages * i8_tile_stage_bytes(bn) + kI8TileEpiBytes + kI8BarrierBytes;
+}
+
+// Where a tile or split starts in its K range: tiles that share a panel would
+// otherwise read the same lines of it at the same moment, and a few lines do not
+// spread over the L2 slices. The integer sum does not depend on the order.
+__device__ __forceinline__ int i8_first_block(int seed, int num_kb) {
+    return num_kb < 16 ? seed % num_kb : seed & 15;
 }
 
 // Tile t of the grouped-M order (the FP16 family's order): groupM row tiles at
@@ -204,7 +194,8 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
             i8_tile_coords(tile, num_m, num_n, p.groupM, tm, tn);
             const int a_row = tm * 256 + int(rank) * 128;
             const int b_row = tn * bn + int(rank) * rows_b;
-            for (int kb = 0; kb < num_kb; ++kb) {
+            int kb = i8_first_block(3 * tm + 5 * tn, num_kb);
+            for (int i = 0; i < num_kb; ++i) {
                 if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.err,
                                kErrTimeoutProducer)) {
                     ok = false;
@@ -215,6 +206,7 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
                 if (leader) mbar_arrive_expect_tx(full_bar(stage), 2 * stage_bytes);
                 tma_load_2d_pair(sa, &tmap_a, fb, kb * kI8BK, a_row);
                 tma_load_2d_pair(sa + 128 * kI8BK, &tmap_b, fb, kb * kI8BK, b_row);
+                if (++kb == num_kb) kb = 0;
                 ++issued;
                 if (++stage == stages) {
                     stage = 0;
@@ -283,8 +275,11 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
         const int quad = warp & 3;
         const int group = epi >> 2;
         const uint32_t tempty0 = map_to_cta(tempty_bar(0), 0);
-        const uint32_t sbuf = epi_base + uint32_t(epi * 4096);
+        const uint32_t sbuf = epi_base + uint32_t(epi * kI8TileStageOut);
         uint8_t* sbuf_ptr = base_ptr + (sbuf - base);
+        // Channel scales and biases of this warp's columns of the tile.
+        float* cols = reinterpret_cast<float*>(base_ptr + (epi_base - base) + 8 * kI8TileStageOut) +
+                      epi * 2 * kI8TileCols;
         const uint32_t row_addr = sbuf + uint32_t(lane * 128);
         const uint32_t sw = uint32_t(lane & 7);
         const T* bias = static_cast<const T*>(p.bias);
@@ -341,12 +336,12 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
             }
         };
         // Integers to values of C in place: r[j] = bits of (float(r[j]) * sb) * sa + bias.
-        auto scale_half = [&](uint32_t (&r)[32], float row_scale, int col0) {
+        auto scale_half = [&](uint32_t (&r)[32], float row_scale, const float* col) {
 #pragma unroll
             for (int g = 0; g < 8; ++g) {
-                const float4 s = load_cols<float>(p.sb, col0 + 4 * g, p.N, p.sb_vec);
+                const float4 s = *reinterpret_cast<const float4*>(col + 4 * g);
                 float4 b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (bias) b = load_cols<T>(bias, col0 + 4 * g, p.N, p.sb_vec);
+                if (bias) b = *reinterpret_cast<const float4*>(col + kI8TileCols + 4 * g);
                 r[4 * g] = __float_as_uint(fmaf(float(int(r[4 * g])) * s.x, row_scale, b.x));
                 r[4 * g + 1] = __float_as_uint(fmaf(float(int(r[4 * g + 1])) * s.y, row_scale, b.y));
                 r[4 * g + 2] = __float_as_uint(fmaf(float(int(r[4 * g + 2])) * s.z, row_scale, b.z));
@@ -359,6 +354,17 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
             i8_tile_coords(tile, num_m, num_n, p.groupM, tm, tn);
             const int row0 = tm * 256 + int(rank) * 128 + quad * 32;
             const float row_scale = row0 + lane < p.M ? p.sa[row0 + lane] : 0.0f;
+            // Fetched while the tile's MMAs still run: read from global memory in
+            // the drain itself they made a 256 x 256 tile's epilogue 6.4 us long.
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < kI8TileCols / 32; ++i) {
+                const int col = tn * bn + (group + 2 * (i / 2)) * 64 + (i % 2) * 32 + lane;
+                const bool in = col < p.N;
+                cols[i * 32 + lane] = in ? p.sb[col] : 0.0f;
+                if (bias) cols[kI8TileCols + i * 32 + lane] = in ? OutType<T>::up(bias[col]) : 0.0f;
+            }
+            __syncwarp();
             int ok = 1;
             if (lane == 0)
                 ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.err, kErrTimeoutEpilogue);
@@ -375,8 +381,9 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
                 tmem_ld_32x32b_x32(taddr + 32, rb);
                 tmem_wait_ld(ra);
                 tmem_wait_ld(rb);
-                scale_half(ra, row_scale, col0);
-                scale_half(rb, row_scale, col0 + 32);
+                const float* col = cols + (u >> 1) * 64;
+                scale_half(ra, row_scale, col);
+                scale_half(rb, row_scale, col + 32);
                 if constexpr (sizeof(T) == 4) {
                     store_staged(ra, row0, col0);
                     if (col0 + 32 < p.N) store_staged(rb, row0, col0 + 32);
@@ -415,15 +422,37 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
 
 constexpr int kI8StreamThreads = 6 * 32;  // producer, MMA, 4 epilogue warps
 
+constexpr int kI8StreamScales = 256 * 4;  // token scales of the tile
+
 __host__ __device__ constexpr int i8_stream_stage_bytes(int bn) { return (128 + bn) * kI8BK; }
 constexpr int i8_stream_smem(int bn, int stages) {
-    return kI8AlignSlack + stages * i8_stream_stage_bytes(bn) + kI8BarrierBytes;
+    return kI8AlignSlack + stages * i8_stream_stage_bytes(bn) + kI8StreamScales + kI8BarrierBytes;
 }
 
-__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
-    int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ int4 ld_cluster_v4(uint32_t addr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
     return v;
+}
+
+// Four values of C at dst, the first `n` of them inside it.
+template <typename T>
+__device__ __forceinline__ void store4(T* dst, float4 v, int n, bool vec) {
+    if (vec && n >= 4) {
+        if constexpr (sizeof(T) == 4)
+            *reinterpret_cast<float4*>(dst) = v;
+        else
+            *reinterpret_cast<uint2*>(dst) =
+                make_uint2(OutType<T>::pack(v.x, v.y), OutType<T>::pack(v.z, v.w));
+        return;
+    }
+    if (n > 0) dst[0] = OutType<T>::down(v.x);
+    if (n > 1) dst[1] = OutType<T>::down(v.y);
+    if (n > 2) dst[2] = OutType<T>::down(v.z);
+    if (n > 3) dst[3] = OutType<T>::down(v.w);
 }
 
 // SPLIT CTAs of one cluster share a tile of 128 channels x bn tokens, each with a
@@ -441,7 +470,8 @@ __global__ void __launch_bounds__(kI8StreamThreads)
     const int stages = p.stages;
     const int bn = p.bn;
     const uint32_t stage_bytes = uint32_t(i8_stream_stage_bytes(bn));
-    const uint32_t bars = base + stages * stage_bytes;
+    const uint32_t bars = base + stages * stage_bytes + kI8StreamScales;
+    float* token_scale = reinterpret_cast<float*>(base_ptr + stages * stage_bytes);
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (kI8MaxStages + s); };
     const uint32_t done_bar = bars + 8u * (2 * kI8MaxStages);
@@ -493,7 +523,8 @@ __global__ void __launch_bounds__(kI8StreamThreads)
         uint32_t phase = 0;
         int issued = 0;
         bool live = true;
-        for (int kb = kb0; kb < kb1; ++kb) {
+        int kb = kb0 + i8_first_block(3 * int(blockIdx.x / SPLIT) + 5 * int(blockIdx.y), kb1 - kb0);
+        for (int i = kb0; i < kb1; ++i) {
             if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.err, kErrTimeoutProducer)) {
                 live = false;
                 break;
@@ -502,6 +533,7 @@ __global__ void __launch_bounds__(kI8StreamThreads)
             mbar_arrive_expect_tx(full_bar(stage), stage_bytes);
             tma_load_2d(sb, &tmap_b, full_bar(stage), kb * kI8BK, f0);
             tma_load_2d(sb + 128 * kI8BK, &tmap_a, full_bar(stage), kb * kI8BK, t0);
+            if (++kb == kb1) kb = kb0;
             ++issued;
             if (++stage == stages) {
                 stage = 0;
@@ -544,75 +576,84 @@ __global__ void __launch_bounds__(kI8StreamThreads)
             mbar_wait(drain_bar, 0, nullptr, p.err, kErrTimeoutDrain);
         }
     } else if (warp >= 2) {
+        for (int i = int(threadIdx.x) - 64; i < bn; i += 128)
+            token_scale[i] = t0 + i < p.M ? p.sa[t0 + i] : 0.0f;
         if (lane == 0) ok = mbar_wait(done_bar, 0, abort_flag, p.err, kErrTimeoutEpilogue);
         ok = __shfl_sync(0xffffffffu, ok, 0);
         tc_fence_after();
-        const int fl = quad * 32 + lane;
-        const int f = f0 + fl;
-        if (ok && SPLIT == 1) {
-            const float channel = f < p.N ? p.sb[f] : 0.0f;
-            const float b = bias && f < p.N ? OutType<T>::up(bias[f]) : 0.0f;
-            for (int c = 0; c < bn && t0 + c < p.M; c += 16) {
-                uint32_t r[16];
-                tmem_ld_32x32b_x16(lane_taddr + uint32_t(c), r);
-                tmem_wait_ld(r);
+        // Every load has landed and every MMA has read it, so the ring can hold
+        // this CTA's sums: token t, channel c at int t * 128 + c.
+        int* part = reinterpret_cast<int*>(base_ptr) + quad * 32 + lane;
+        for (int c = 0; ok && c < bn && t0 + c < p.M; c += 16) {
+            uint32_t r[16];
+            tmem_ld_32x32b_x16(lane_taddr + uint32_t(c), r);
+            tmem_wait_ld(r);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int t = t0 + c + i;
-                    if (t < p.M && f < p.N)
-                        C[(long long)t * p.ldc + f] = OutType<T>::down(
-                            fmaf(float(int(r[i])) * channel, p.sa[t], b));
-                }
-            }
-        } else if (ok) {
-            // Every load has landed and every MMA has read it, so the ring can
-            // hold this CTA's sums: token t, channel fl at int t * 128 + fl.
-            int* part = reinterpret_cast<int*>(base_ptr);
-            for (int c = 0; c < bn && t0 + c < p.M; c += 16) {
-                uint32_t r[16];
-                tmem_ld_32x32b_x16(lane_taddr + uint32_t(c), r);
-                tmem_wait_ld(r);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) part[(c + i) * 128 + fl] = int(r[i]);
-            }
+            for (int i = 0; i < 16; ++i) part[(c + i) * 128] = int(r[i]);
         }
     }
 
     tc_fence_before();
     __syncwarp();
-    if constexpr (SPLIT > 1) {
+    if constexpr (SPLIT > 1)
         cluster_sync();  // every rank's sums are in its shared memory
-        if (warp >= 2 && ok) {
-            const int fl = quad * 32 + lane;
-            const int f = f0 + fl;
-            const float channel = f < p.N ? p.sb[f] : 0.0f;
-            const float b = bias && f < p.N ? OutType<T>::up(bias[f]) : 0.0f;
-            const int live = min(bn, p.M - t0);  // tokens of this tile
-            uint32_t peer[SPLIT];
+    else
+        __syncthreads();
+    if (warp >= 2 && ok) {
+        // A warp takes whole tokens, four channels to a lane, so that the sums
+        // are read and C is written in full lines; the tokens are dealt to the
+        // ranks and their warps in turn, four at a time in flight.
+        const int f = f0 + lane * 4;
+        const int in = p.N - f;  // channels of this lane inside C
+        float4 channel, b;
+        channel.x = in > 0 ? p.sb[f] : 0.0f;
+        channel.y = in > 1 ? p.sb[f + 1] : 0.0f;
+        channel.z = in > 2 ? p.sb[f + 2] : 0.0f;
+        channel.w = in > 3 ? p.sb[f + 3] : 0.0f;
+        b.x = bias && in > 0 ? OutType<T>::up(bias[f]) : 0.0f;
+        b.y = bias && in > 1 ? OutType<T>::up(bias[f + 1]) : 0.0f;
+        b.z = bias && in > 2 ? OutType<T>::up(bias[f + 2]) : 0.0f;
+        b.w = bias && in > 3 ? OutType<T>::up(bias[f + 3]) : 0.0f;
+        const int live = min(bn, p.M - t0);  // tokens of this tile
+        uint32_t peer[SPLIT];
 #pragma unroll
-            for (int s = 0; s < SPLIT; ++s) peer[s] = map_to_cta(base + uint32_t(fl * 4), s);
-            // Tokens are dealt to the ranks in turn, four at a time in flight.
-            for (int t = rank; t < live; t += 4 * SPLIT) {
-                int sum[4];
+        for (int s = 0; s < SPLIT; ++s)
+            peer[s] = SPLIT > 1 ? map_to_cta(base + uint32_t(lane * 16), s)
+                                : base + uint32_t(lane * 16);
+        constexpr int kStep = 4 * SPLIT;  // tokens between two of one warp's
+        constexpr int kFlight = SPLIT >= 8 ? 2 : 4;
+        for (int t = rank + (warp - 2) * SPLIT; t < live; t += kFlight * kStep) {
+            int4 sum[kFlight];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    sum[i] = 0;
-                    const int ti = t + i * SPLIT;
-                    if (ti < live) {
+            for (int i = 0; i < kFlight; ++i) {
+                const int ti = t + i * kStep;
+                sum[i] = make_int4(0, 0, 0, 0);
+                if (ti < live) {
 #pragma unroll
-                        for (int s = 0; s < SPLIT; ++s)
-                            sum[i] += ld_cluster_s32(peer[s] + uint32_t(ti) * 512u);
+                    for (int s = 0; s < SPLIT; ++s) {
+                        const int4 v = ld_cluster_v4(peer[s] + uint32_t(ti) * 512u);
+                        sum[i].x += v.x;
+                        sum[i].y += v.y;
+                        sum[i].z += v.z;
+                        sum[i].w += v.w;
                     }
                 }
+            }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int ti = t + i * SPLIT;
-                    if (ti < live && f < p.N)
-                        C[(long long)(t0 + ti) * p.ldc + f] = OutType<T>::down(
-                            fmaf(float(sum[i]) * channel, p.sa[t0 + ti], b));
-                }
+            for (int i = 0; i < kFlight; ++i) {
+                const int ti = t + i * kStep;
+                if (ti >= live) break;
+                const float token = token_scale[ti];
+                float4 v;
+                v.x = fmaf(float(sum[i].x) * channel.x, token, b.x);
+                v.y = fmaf(float(sum[i].y) * channel.y, token, b.y);
+                v.z = fmaf(float(sum[i].z) * channel.z, token, b.z);
+                v.w = fmaf(float(sum[i].w) * channel.w, token, b.w);
+                store4<T>(C + (long long)(t0 + ti) * p.ldc + f, v, in, p.vec_store);
             }
         }
+    }
+    if constexpr (SPLIT > 1) {
         __syncwarp();
         cluster_sync();  // no rank leaves while another reads its sums
     } else {
