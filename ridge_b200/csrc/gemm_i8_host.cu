@@ -20,6 +20,9 @@ namespace {
 
 constexpr int kMaxDevices = 64;
 constexpr int kMaxDynSmem = 232448;  // 227 KB opt-in limit per CTA on sm_100
+constexpr int kSmemPerSm = 233472;   // 228 KB per SM
+constexpr int kSmemReservedPerCta = 1024;
+constexpr int kTmemColsPerSm = 512;
 
 // K = 0: no sum, C is the bias (a non-finite scale still makes its row or column NaN).
 template <typename T>
@@ -35,42 +38,127 @@ __global__ void ridge_gemm_i8_empty(const I8Params p) {
 // One launch: which kernel, its tile and its ring.
 struct Plan {
     bool stream;
-    int bn, stages, split;
+    int bn, stages;
+    int split;        // stream: CTAs of a cluster that share K
+    int64_t items;    // units of work: tiles and strips, or CTAs of the streaming kernel
+    int whole, cut;   // tile: see I8Params
 };
 
-int ceil_div(int64_t a, int64_t b) { return int((a + b - 1) / b); }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 int stages_for(int stage_bytes, int fixed, int budget) {
     return std::min(kI8MaxStages, (budget - fixed) / stage_bytes);
 }
 
-Plan make_plan(int64_t M, int64_t N, int64_t K, int num_sms) {
+// The tile kernel's grid for tiles bn wide on `pairs` resident pairs: full rounds
+// of whole tiles, and a last round whose tiles are cut into as many strips (of
+// whole 64 columns) as there are pairs to take them.
+Plan tile_plan(int64_t M, int64_t N, int bn, int pairs) {
     Plan p{};
-    const int num_kb = ceil_div(K, kI8BK);
+    p.bn = bn;
+    p.stages = stages_for(i8_tile_stage_bytes(bn), i8_tile_smem(bn, 0), kMaxDynSmem);
+    p.split = 1;
+    const int64_t tiles = ceil_div(M, 256) * ceil_div(N, bn);
+    const int64_t last = tiles % pairs;
+    p.cut = 1;
+    for (int cut = 2; last > 0 && cut <= bn / 64; ++cut)
+        if (bn % (64 * cut) == 0 && last * cut <= pairs) p.cut = cut;
+    p.whole = int(p.cut > 1 ? tiles - last : tiles);
+    p.items = p.whole + (tiles - p.whole) * p.cut;
+    return p;
+}
+
+// CTAs of the streaming kernel that share an SM with this ring.
+int stream_residents(int bn, int stages) {
+    int cols = 32;
+    while (cols < bn) cols *= 2;
+    const int by_smem = kSmemPerSm / (i8_stream_smem(bn, stages) + kSmemReservedPerCta);
+    return std::max(1, std::min(by_smem, kTmemColsPerSm / cols));
+}
+
+// Up to `bn` tokens to a tile, evened out over the tiles, and the ring: all of
+// the shared memory when every CTA can have an SM to itself, else half of it
+// where that leaves three stages.
+Plan stream_plan(int64_t M, int64_t N, int bn, int split, int num_sms) {
+    Plan p{};
+    p.stream = true;
+    p.split = split;
+    const int64_t token_tiles = ceil_div(M, bn);
+    p.bn = int(ceil_div(ceil_div(M, token_tiles), 16) * 16);
+    p.items = ceil_div(N, 128) * ceil_div(M, p.bn) * split;
+    const int fixed = i8_stream_smem(p.bn, 0), stage = i8_stream_stage_bytes(p.bn);
+    p.stages = stages_for(stage, fixed, kMaxDynSmem);
+    if (p.items > num_sms) {
+        const int half = stages_for(stage, fixed, kSmemPerSm / 2 - kSmemReservedPerCta);
+        if (half >= 3) p.stages = half;
+    }
+    return p;
+}
+
+// Estimated times in microseconds, good for ranking plans: fitted to 2,656 timed
+// launches of 107 shapes (1 to 8192 tokens, K of 256 to 16384, every tile, split
+// and ring below). The plan they pick is on average 1.5% slower than the best of a
+// shape, 12% at worst.
+//
+// A streaming CTA takes 0.26 us for a K block of its own and an SM takes in
+// 97 bytes/ns for all of its CTAs; sums leave at 20 ns a token, over a cluster
+// with 1 us + 70 ns a rank for the exchange. Clusters of 4 and 8 do not find
+// room on every SM.
+double stream_time(const Plan& p, int64_t num_kb, int num_sms) {
+    const double room = p.split == 8 ? 0.757 : p.split == 4 ? 0.892 : 1.0;
+    const int64_t at_once = std::max<int64_t>(
+        1, int64_t(stream_residents(p.bn, p.stages) * room * num_sms));
+    const int64_t waves = ceil_div(p.items, at_once);
+    const int64_t per_sm = std::max(waves, ceil_div(p.items, num_sms));
+    const double steps = double(ceil_div(num_kb, p.split));
+    const double out = (p.split > 1 ? 1.0 + 0.07 * p.split : 0.25) + 0.02 * p.bn;
+    const double feed = i8_stream_stage_bytes(p.bn) / 97e3;
+    return 4.2 + waves * out + steps * std::max(0.26 * waves, feed * per_sm);
+}
+
+// A pair takes 0.35 to 0.38 us for a K block, little less for narrow tiles.
+double tile_time(const Plan& p, int64_t num_kb, int pairs) {
+    auto step = [](int width) { return width == 256 ? 0.38 : width == 192 ? 0.36 : 0.35; };
+    const int64_t rounds = p.cut > 1 ? p.whole / pairs : ceil_div(p.items, pairs);
+    double t = 7.4 + double(rounds) * num_kb * step(p.bn);
+    if (p.cut > 1) t += num_kb * step(p.bn / p.cut);
+    return t;
+}
+
+// The kernel and tile with the least estimated time. Sums are exact integers, so
+// results do not depend on the choice.
+Plan make_plan(int64_t M, int64_t N, int64_t K, int num_sms, int pairs) {
 #ifdef RIDGE_I8_PROBE
     if (const char* v = std::getenv("RIDGE_I8_PLAN")) {
-        int s = 0;
-        std::sscanf(v, "%d,%d,%d,%d", &s, &p.bn, &p.stages, &p.split);
-        p.stream = s != 0;
-        if (p.stream) p.bn = std::min(p.bn, ceil_div(M, 16) * 16);
+        int s = 0, bn = 0, stages = 0, split = 0;
+        std::sscanf(v, "%d,%d,%d,%d", &s, &bn, &stages, &split);
+        Plan p = s ? stream_plan(M, N, bn, split, num_sms) : tile_plan(M, N, bn, pairs);
+        p.stages = stages;
         return p;
     }
 #endif
-    if (M <= 256) {
-        p.stream = true;
-        p.bn = ceil_div(M, 16) * 16;
-        const int tiles = ceil_div(N, 128);
-        p.split = 1;
-        while (p.split < 8 && tiles * p.split * 2 <= num_sms && num_kb >= p.split * 2 * 4)
-            p.split *= 2;
-        p.stages = stages_for(i8_stream_stage_bytes(p.bn), i8_stream_smem(0, 0), kMaxDynSmem);
-        return p;
+    const int64_t num_kb = ceil_div(K, kI8BK);
+    Plan best{};
+    double best_time = 0;
+    auto offer = [&](const Plan& p, double t) {
+        if (best.bn == 0 || t < best_time) {
+            best = p;
+            best_time = t;
+        }
+    };
+    for (int bn : {256, 192, 128, 64}) {
+        const Plan p = tile_plan(M, N, bn, pairs);
+        offer(p, tile_time(p, num_kb, pairs));
     }
-    p.stream = false;
-    p.bn = 256;
-    p.stages = stages_for(i8_tile_stage_bytes(p.bn), i8_tile_smem(p.bn, 0), kMaxDynSmem);
-    p.split = 1;
-    return p;
+    for (int bn : {64, 128, 256}) {
+        if (ceil_div(M, bn) > 65535) continue;  // the grid's second dimension
+        for (int split = 1; split <= 8 && split <= num_kb; split *= 2) {
+            const Plan p = stream_plan(M, N, bn, split, num_sms);
+            offer(p, stream_time(p, num_kb, num_sms));
+        }
+        if (M <= bn) break;  // one token tile already
+    }
+    return best;
 }
 
 // rows x cols bytes, pitch ld, read in boxes of box_rows x 128 bytes.
@@ -126,49 +214,40 @@ void set_cluster(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, unsigned ct
     cfg->numAttrs = 1;
 }
 
+// Pairs of the tile kernel that run at once (for the full shared memory, one CTA
+// per SM). The two CTAs of a pair sit on one TPC, so it is asked of the runtime.
 template <typename T>
-int launch_tile(const Plan& plan, const CUtensorMap& a, const CUtensorMap& b,
-                const CUtensorMap& c, const I8Params& p, const DeviceInfo& dev,
-                cudaStream_t stream) {
+int resident_pairs(const DeviceInfo& dev, int* pairs) {
     static std::atomic<bool> ready[kMaxDevices];
-    static std::atomic<int> pairs[kMaxDevices];  // 0 = not asked yet
+    static std::atomic<int> known[kMaxDevices];  // 0 = not asked yet
     const void* func = reinterpret_cast<const void*>(&ridge_gemm_i8_tile<T>);
     const int st = allow_smem(func, &ready[dev.device]);
     if (st != RIDGE_OK) return st;
+    *pairs = known[dev.device].load(std::memory_order_relaxed);
+    if (*pairs > 0) return RIDGE_OK;
     cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(4);
     cfg.blockDim = dim3(kI8TileThreads);
-    cfg.dynamicSmemBytes = size_t(i8_tile_smem(plan.bn, plan.stages));
-    cfg.stream = stream;
+    cfg.dynamicSmemBytes = kMaxDynSmem;
     cudaLaunchAttribute attr[1];
     set_cluster(&cfg, attr, 2);
-    // The two CTAs of a pair sit on one TPC, so how many pairs run at once is
-    // asked of the runtime (for the full shared memory: one CTA per SM).
-    int units = pairs[dev.device].load(std::memory_order_relaxed);
-    if (units == 0) {
-        cudaLaunchConfig_t q = cfg;
-        q.gridDim = dim3(4);
-        q.dynamicSmemBytes = kMaxDynSmem;
-        if (cudaOccupancyMaxActiveClusters(&units, func, &q) != cudaSuccess || units <= 0) {
-            cudaGetLastError();
-            units = dev.num_sms / 2;
-        }
-        pairs[dev.device].store(units, std::memory_order_relaxed);
+    if (cudaOccupancyMaxActiveClusters(pairs, func, &cfg) != cudaSuccess || *pairs <= 0) {
+        cudaGetLastError();
+        *pairs = std::max(1, dev.num_sms / 2);
     }
-    const int64_t tiles = int64_t(ceil_div(p.M, 256)) * ceil_div(p.N, plan.bn);
-    if (tiles > int64_t(1) << 30) return RIDGE_EINVAL;
-    cfg.gridDim = dim3(unsigned(std::min<int64_t>(tiles, units)) * 2);
-    return int(cudaLaunchKernelEx(&cfg, ridge_gemm_i8_tile<T>, a, b, c, p));
+    known[dev.device].store(*pairs, std::memory_order_relaxed);
+    return RIDGE_OK;
 }
 
 template <typename T, int SPLIT>
-int launch_stream_n(const Plan& plan, const CUtensorMap& a, const CUtensorMap& b,
+int launch_stream(const Plan& plan, const CUtensorMap& a, const CUtensorMap& b,
                     const I8Params& p, const DeviceInfo& dev, cudaStream_t stream) {
     static std::atomic<bool> ready[kMaxDevices];
     const int st = allow_smem(reinterpret_cast<const void*>(&ridge_gemm_i8_stream<T, SPLIT>),
                               &ready[dev.device]);
     if (st != RIDGE_OK) return st;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(ceil_div(p.N, 128)) * SPLIT, unsigned(ceil_div(p.M, plan.bn)));
+    cfg.gridDim = dim3(unsigned(ceil_div(p.N, 128) * SPLIT), unsigned(ceil_div(p.M, plan.bn)));
     if (cfg.gridDim.y > 65535) return RIDGE_EINVAL;
     cfg.blockDim = dim3(kI8StreamThreads);
     cfg.dynamicSmemBytes = size_t(i8_stream_smem(plan.bn, plan.stages));
@@ -179,23 +258,59 @@ int launch_stream_n(const Plan& plan, const CUtensorMap& a, const CUtensorMap& b
 }
 
 template <typename T>
-int launch_typed(const Plan& plan, const CUtensorMap& a, const CUtensorMap& b,
-                 const CUtensorMap& c, const I8Params& p, const DeviceInfo& dev,
-                 cudaStream_t stream) {
-    if (!plan.stream) return launch_tile<T>(plan, a, b, c, p, dev, stream);
-    switch (plan.split) {
-        case 1: return launch_stream_n<T, 1>(plan, a, b, p, dev, stream);
-        case 2: return launch_stream_n<T, 2>(plan, a, b, p, dev, stream);
-        case 4: return launch_stream_n<T, 4>(plan, a, b, p, dev, stream);
-        default: return launch_stream_n<T, 8>(plan, a, b, p, dev, stream);
-    }
-}
-
-template <typename T>
 int launch_empty(const I8Params& p, cudaStream_t stream) {
     const dim3 grid(unsigned(ceil_div(p.N, 256)), unsigned(std::min(p.M, 65535)));
     ridge_gemm_i8_empty<T><<<grid, 256, 0, stream>>>(p);
     return int(cudaGetLastError());
+}
+
+template <typename T>
+int run_product(const int8_t* A, const int8_t* B, int32_t type, int64_t lda, int64_t ldb,
+                I8Params p, const DeviceInfo& dev, cudaStream_t stream) {
+    int pairs = 0;
+    int st = resident_pairs<T>(dev, &pairs);
+    if (st != RIDGE_OK) return st;
+    const Plan plan = make_plan(p.M, p.N, p.K, dev.num_sms, pairs);
+    p.bn = plan.bn;
+    p.stages = plan.stages;
+    CUtensorMap a, b;
+    st = operand_map(&a, A, p.M, p.K, lda, plan.stream ? plan.bn : 128);
+    if (st != RIDGE_OK) return st;
+    st = operand_map(&b, B, p.N, p.K, ldb, plan.stream ? 128 : plan.bn / 2);
+    if (st != RIDGE_OK) return st;
+    if (plan.stream) {
+        p.vec_store = reinterpret_cast<uintptr_t>(p.C) % (4 * sizeof(T)) == 0 && p.ldc % 4 == 0;
+        switch (plan.split) {
+            case 1: return launch_stream<T, 1>(plan, a, b, p, dev, stream);
+            case 2: return launch_stream<T, 2>(plan, a, b, p, dev, stream);
+            case 4: return launch_stream<T, 4>(plan, a, b, p, dev, stream);
+            default: return launch_stream<T, 8>(plan, a, b, p, dev, stream);
+        }
+    }
+    if (plan.items > int64_t(1) << 30) return RIDGE_EINVAL;
+    p.groupM = 8;
+    p.whole = plan.whole;
+    p.cut = plan.cut;
+    CUtensorMap strip = b, c;
+    if (plan.cut > 1) {
+        st = operand_map(&strip, B, p.N, p.K, ldb, plan.bn / plan.cut / 2);
+        if (st != RIDGE_OK) return st;
+    }
+    // Stores through the tensor map need 16-byte aligned rows of C.
+    std::memset(&c, 0, sizeof(c));
+    p.tma_store = (reinterpret_cast<uintptr_t>(p.C) & 15) == 0 && (p.ldc * sizeof(T)) % 16 == 0;
+    if (p.tma_store) {
+        st = output_map(&c, p.C, type, p.M, p.N, p.ldc);
+        if (st != RIDGE_OK) return st;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(std::min<int64_t>(plan.items, pairs)) * 2);
+    cfg.blockDim = dim3(kI8TileThreads);
+    cfg.dynamicSmemBytes = size_t(i8_tile_smem(plan.bn, plan.stages));
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    set_cluster(&cfg, attr, 2);
+    return int(cudaLaunchKernelEx(&cfg, ridge_gemm_i8_tile<T>, a, b, strip, c, p));
 }
 
 }  // namespace
@@ -249,26 +364,8 @@ extern "C" int ridge_gemm_i8(const int8_t* A, const float* scale_a, const int8_t
                : type == RIDGE_BF16 ? launch_empty<__nv_bfloat16>(p, stream)
                                     : launch_empty<float>(p, stream);
 
-    const Plan plan = make_plan(M, N, K, dev.num_sms);
-    p.bn = plan.bn;
-    p.stages = plan.stages;
-    p.groupM = 8;
-    p.vec_store = reinterpret_cast<uintptr_t>(C) % uintptr_t(4 * size) == 0 && ldc % 4 == 0;
-    // Stores through the tensor map need 16-byte aligned rows of C.
-    p.tma_store = (reinterpret_cast<uintptr_t>(C) & 15) == 0 && (ldc * size) % 16 == 0;
-    CUtensorMap tmap_a, tmap_b, tmap_c;
-    std::memset(&tmap_c, 0, sizeof(tmap_c));
-    st = operand_map(&tmap_a, A, M, K, lda, plan.stream ? plan.bn : 128);
-    if (st != RIDGE_OK) return st;
-    st = operand_map(&tmap_b, B, N, K, ldb, plan.stream ? 128 : plan.bn / 2);
-    if (st != RIDGE_OK) return st;
-    if (!plan.stream && p.tma_store) {
-        st = output_map(&tmap_c, C, type, M, N, ldc);
-        if (st != RIDGE_OK) return st;
-    }
-    if (type == RIDGE_F16)
-        return launch_typed<__half>(plan, tmap_a, tmap_b, tmap_c, p, dev, stream);
+    if (type == RIDGE_F16) return run_product<__half>(A, B, type, lda, ldb, p, dev, stream);
     if (type == RIDGE_BF16)
-        return launch_typed<__nv_bfloat16>(plan, tmap_a, tmap_b, tmap_c, p, dev, stream);
-    return launch_typed<float>(plan, tmap_a, tmap_b, tmap_c, p, dev, stream);
+        return run_product<__nv_bfloat16>(A, B, type, lda, ldb, p, dev, stream);
+    return run_product<float>(A, B, type, lda, ldb, p, dev, stream);
 }

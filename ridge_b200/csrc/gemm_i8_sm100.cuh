@@ -52,6 +52,8 @@ struct I8Params {
     int M, N, K;
     long long ldc;
     int bn;         // tile: columns of C per tile (64, 128, 192, 256); stream: rows of A (16..256)
+    int whole;      // tile: tiles computed bn wide; each later one is cut into `cut` narrower
+    int cut;        // ones (1, 2 or 4, widths of whole 64s) that fill the last round
     int stages;
     int groupM;
     int tma_store;  // tile: C is stored through its tensor map; 0: from shared memory by threads
@@ -87,7 +89,7 @@ struct OutType<float> {
 
 // ------------------------------------------------------------------ tiles by 2-CTA pairs
 
-constexpr int kI8TileThreads = 10 * 32;  // producer, MMA, 8 epilogue warps
+constexpr int kI8TileThreads = 11 * 32;  // A producer, MMA, 8 epilogue warps, B producer
 constexpr int kI8TileStageOut = 4096;  // 32 rows x 128 bytes of C per epilogue warp
 constexpr int kI8TileCols = 2 * 64;    // columns of a tile that one epilogue warp drains
 constexpr int kI8TileEpiBytes = 8 * (kI8TileStageOut + kI8TileCols * 8);
@@ -99,6 +101,15 @@ constexpr int i8_tile_smem(int bn, int stages) {
     return kI8AlignSlack + stages * i8_tile_stage_bytes(bn) + kI8TileEpiBytes + kI8BarrierBytes;
 }
 
+// Abort path of a producer: its loads in flight (which take microseconds) land
+// before the CTA can exit. A timed wait, since the stage they complete may never
+// be armed once the other producer has given up too.
+__device__ __forceinline__ void i8_let_loads_land() {
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 2000000ull) {
+    }
+}
+
 // Where a tile or split starts in its K range: tiles that share a panel would
 // otherwise read the same lines of it at the same moment, and a few lines do not
 // spread over the L2 slices. The integer sum does not depend on the order.
@@ -106,23 +117,40 @@ __device__ __forceinline__ int i8_first_block(int seed, int num_kb) {
     return num_kb < 16 ? seed % num_kb : seed & 15;
 }
 
-// Tile t of the grouped-M order (the FP16 family's order): groupM row tiles at
-// a time, column by column inside the group.
-__device__ __forceinline__ void i8_tile_coords(int tile, int num_m, int num_n, int groupM, int& tm,
-                                               int& tn) {
-    const int per_group = groupM * num_n;
+// One unit of work of the tile kernel: rows from 256 * tm, columns [col, col + width).
+struct I8Item {
+    int tm, tn, col, width;
+};
+
+// Item i: the tiles in grouped-M order (the FP16 family's: groupM row tiles at a
+// time, column by column inside the group), those from `whole` on cut into
+// column strips. A last round of few tiles then takes all pairs for less than a
+// tile's time instead of a few pairs for all of it.
+__device__ __forceinline__ bool i8_item(const I8Params& p, int i, int num_m, int num_n, I8Item& w) {
+    int tile = i, strip = 0, cut = 1;
+    if (i >= p.whole) {
+        cut = p.cut;
+        tile = p.whole + (i - p.whole) / cut;
+        strip = (i - p.whole) % cut;
+    }
+    if (tile >= num_m * num_n) return false;
+    const int per_group = p.groupM * num_n;
     const int group = tile / per_group;
-    const int first_m = group * groupM;
-    const int rows = min(num_m - first_m, groupM);
+    const int first_m = group * p.groupM;
+    const int rows = min(num_m - first_m, p.groupM);
     const int in_group = tile - group * per_group;
-    tm = first_m + in_group % rows;
-    tn = in_group / rows;
+    w.tm = first_m + in_group % rows;
+    w.tn = in_group / rows;
+    w.width = p.bn / cut;
+    w.col = w.tn * p.bn + strip * w.width;
+    return true;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kI8TileThreads, 1)
     ridge_gemm_i8_tile(const __grid_constant__ CUtensorMap tmap_a,
                        const __grid_constant__ CUtensorMap tmap_b,
+                       const __grid_constant__ CUtensorMap tmap_strip,
                        const __grid_constant__ CUtensorMap tmap_c, const I8Params p) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = smem_u32(smem_raw);
@@ -131,7 +159,6 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
 
     const int stages = p.stages;
     const int bn = p.bn;
-    const int rows_b = bn / 2;  // rows of B held by this CTA
     const uint32_t stage_bytes = uint32_t(i8_tile_stage_bytes(bn));
     const uint32_t epi_base = base + stages * stage_bytes;
     const uint32_t bars = epi_base + kI8TileEpiBytes;
@@ -177,24 +204,28 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
 
     const int num_m = (p.M + 255) / 256;
     const int num_n = (p.N + bn - 1) / bn;
-    const int num_tiles = num_m * num_n;
     const int num_kb = (p.K + kI8BK - 1) / kI8BK;
     const int unit = blockIdx.x / 2;
     const int num_units = gridDim.x / 2;
 
-    if (warp == 0 && lane == 0) {
-        // ------------------------------------------------------ TMA producer
+    if ((warp == 0 || warp == 10) && lane == 0) {
+        // ------------------------------------------------------ TMA producers
+        // Warp 0 loads A and arms the stage, warp 10 loads B. A load may complete
+        // before its phase is armed; the phase cannot finish before the arming
+        // thread arrives.
+        const bool loads_a = warp == 0;
         const uint32_t leader_full0 = map_to_cta(full_bar(0), 0);
         int stage = 0;
         uint32_t phase = 0;
-        long long issued = 0;
         bool ok = true;
-        for (int tile = unit; ok && tile < num_tiles; tile += num_units) {
-            int tm, tn;
-            i8_tile_coords(tile, num_m, num_n, p.groupM, tm, tn);
-            const int a_row = tm * 256 + int(rank) * 128;
-            const int b_row = tn * bn + int(rank) * rows_b;
-            int kb = i8_first_block(3 * tm + 5 * tn, num_kb);
+        I8Item w;
+        for (int it = unit; ok && i8_item(p, it, num_m, num_n, w); it += num_units) {
+            const int rows_b = w.width / 2;  // rows of B held by this CTA
+            const int a_row = w.tm * 256 + int(rank) * 128;
+            const int b_row = w.col + int(rank) * rows_b;
+            const void* map_b = w.width == bn ? &tmap_b : &tmap_strip;
+            const uint32_t bytes = uint32_t(i8_tile_stage_bytes(w.width));
+            int kb = i8_first_block(3 * w.tm + 5 * w.tn, num_kb);
             for (int i = 0; i < num_kb; ++i) {
                 if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.err,
                                kErrTimeoutProducer)) {
@@ -203,70 +234,70 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
                 }
                 const uint32_t sa = base + stage * stage_bytes;
                 const uint32_t fb = leader_full0 + 8u * uint32_t(stage);
-                if (leader) mbar_arrive_expect_tx(full_bar(stage), 2 * stage_bytes);
-                tma_load_2d_pair(sa, &tmap_a, fb, kb * kI8BK, a_row);
-                tma_load_2d_pair(sa + 128 * kI8BK, &tmap_b, fb, kb * kI8BK, b_row);
+                if (loads_a) {
+                    if (leader) mbar_arrive_expect_tx(full_bar(stage), 2 * bytes);
+                    tma_load_2d_pair(sa, &tmap_a, fb, kb * kI8BK, a_row);
+                } else {
+                    tma_load_2d_pair(sa + 128 * kI8BK, map_b, fb, kb * kI8BK, b_row);
+                }
                 if (++kb == num_kb) kb = 0;
-                ++issued;
                 if (++stage == stages) {
                     stage = 0;
                     phase ^= 1u;
                 }
             }
         }
-        if (!ok && leader) {
-            // Abort path: loads in flight land before the pair can exit (the
-            // leader's barriers count the follower's bytes too).
-            const long long first = issued > stages ? issued - stages : 0;
-            for (long long i = first; i < issued; ++i)
-                mbar_wait(full_bar(int(i % stages)), uint32_t((i / stages) & 1), nullptr, p.err,
-                          kErrTimeoutDrain);
-        }
-    } else if (warp == 1 && lane == 0 && leader) {
+        if (!ok) i8_let_loads_land();
+    } else if (warp == 1 && leader) {
         // ------------------------------------------------------ MMA issuer
-        const uint32_t idesc = make_idesc_i8_s32(256, bn);
+        // The whole warp walks the ring and one elected lane issues: with every
+        // address warp-uniform an MMA takes a few instructions to issue, against
+        // about 75 cycles each from a lane that the compiler sees as divergent.
         int stage = 0;
         uint32_t phase = 0;
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
-        for (int tile = unit; ok && tile < num_tiles; tile += num_units) {
-            if (!mbar_wait<true>(tempty_bar(acc), acc_phase ^ 1u, abort_flag, p.err,
-                                 kErrTimeoutMma)) {
-                ok = false;
-                break;
-            }
+        I8Item w;
+        for (int it = unit; ok && i8_item(p, it, num_m, num_n, w); it += num_units) {
+            const uint32_t idesc = make_idesc_i8_s32(256, w.width);
+            ok = __all_sync(0xffffffffu, mbar_wait<true>(tempty_bar(acc), acc_phase ^ 1u,
+                                                         abort_flag, p.err, kErrTimeoutMma));
+            if (!ok) break;
             tc_fence_after();
             const uint32_t d = tmem_base + uint32_t(acc * 256);
             for (int kb = 0; kb < num_kb; ++kb) {
-                if (!mbar_wait(full_bar(stage), phase, abort_flag, p.err, kErrTimeoutMma)) {
-                    ok = false;
-                    break;
-                }
+                ok = __all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, abort_flag, p.err,
+                                                       kErrTimeoutMma));
+                if (!ok) break;
                 tc_fence_after();
                 const uint32_t sa = base + stage * stage_bytes;
-                const uint32_t sb = sa + 128 * kI8BK;
+                const uint64_t da = make_smem_desc<128>(sa);
+                const uint64_t db = make_smem_desc<128>(sa + 128 * kI8BK);
+                if (elect_one()) {
 #pragma unroll
-                for (int kk = 0; kk < kI8BK / 32; ++kk)
-                    umma_i8<2>(d, make_smem_desc<128>(sa + kk * 32),
-                               make_smem_desc<128>(sb + kk * 32), idesc,
-                               (kb > 0 || kk > 0) ? 1u : 0u);
-                umma_commit_pair(empty_bar(stage), 0x3);
+                    for (int kk = 0; kk < kI8BK / 32; ++kk)  // 32 bytes on: 2 in address >> 4
+                        umma_i8<2>(d, da + 2 * kk, db + 2 * kk, idesc,
+                                   (kb > 0 || kk > 0) ? 1u : 0u);
+                    umma_commit_pair(empty_bar(stage), 0x3);
+                }
+                __syncwarp();
                 if (++stage == stages) {
                     stage = 0;
                     phase ^= 1u;
                 }
             }
             if (!ok) break;
-            umma_commit_pair(tfull_bar(acc), 0x3);
+            if (elect_one()) umma_commit_pair(tfull_bar(acc), 0x3);
+            __syncwarp();
             acc ^= 1;
             if (acc == 0) acc_phase ^= 1u;
         }
-        if (!ok) {
+        if (!ok && elect_one()) {
             umma_commit_pair(drain_bar, 0x1);
             mbar_wait(drain_bar, 0, nullptr, p.err, kErrTimeoutDrain);
         }
-    } else if (warp >= 2) {
+    } else if (warp >= 2 && warp < 10) {
         // ------------------------------------------------------ epilogue
         // A warp drains 32 rows x 64 columns at a time (two column groups of four
         // warps take alternate 64s): TMEM -> registers -> scaled -> 4 KB of
@@ -284,7 +315,6 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
         const uint32_t sw = uint32_t(lane & 7);
         const T* bias = static_cast<const T*>(p.bias);
         T* C = static_cast<T*>(p.C);
-        const int units = bn / 64;
         int acc = 0;
         uint32_t acc_phase = 0;
 
@@ -323,8 +353,8 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
                     const uint32_t off =
                         uint32_t(r * 128) +
                         (((uint32_t(lane >> 2)) ^ uint32_t(r & 7)) << 4) + uint32_t((lane & 3) * 4);
-                    const uint32_t w = *reinterpret_cast<const uint32_t*>(sbuf_ptr + off);
-                    const T* e = reinterpret_cast<const T*>(&w);
+                    const uint32_t bits = *reinterpret_cast<const uint32_t*>(sbuf_ptr + off);
+                    const T* e = reinterpret_cast<const T*>(&bits);
                     T* dst = C + (long long)(row0 + r) * p.ldc;
 #pragma unroll
                     for (int i = 0; i < kPer; ++i) {
@@ -349,17 +379,17 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
             }
         };
 
-        for (int tile = unit; tile < num_tiles; tile += num_units) {
-            int tm, tn;
-            i8_tile_coords(tile, num_m, num_n, p.groupM, tm, tn);
-            const int row0 = tm * 256 + int(rank) * 128 + quad * 32;
+        I8Item w;
+        for (int it = unit; i8_item(p, it, num_m, num_n, w); it += num_units) {
+            const int units = w.width / 64;
+            const int row0 = w.tm * 256 + int(rank) * 128 + quad * 32;
             const float row_scale = row0 + lane < p.M ? p.sa[row0 + lane] : 0.0f;
             // Fetched while the tile's MMAs still run: read from global memory in
             // the drain itself they made a 256 x 256 tile's epilogue 6.4 us long.
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < kI8TileCols / 32; ++i) {
-                const int col = tn * bn + (group + 2 * (i / 2)) * 64 + (i % 2) * 32 + lane;
+                const int col = w.col + (group + 2 * (i / 2)) * 64 + (i % 2) * 32 + lane;
                 const bool in = col < p.N;
                 cols[i * 32 + lane] = in ? p.sb[col] : 0.0f;
                 if (bias) cols[kI8TileCols + i * 32 + lane] = in ? OutType<T>::up(bias[col]) : 0.0f;
@@ -372,7 +402,7 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
             if (!ok) break;
             tc_fence_after();
             for (int u = group; u < units; u += 2) {
-                const int col0 = tn * bn + u * 64;
+                const int col0 = w.col + u * 64;
                 if (row0 >= p.M || col0 >= p.N) break;  // nothing of this warp's is in C
                 uint32_t ra[32], rb[32];
                 const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) +
@@ -420,21 +450,26 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
 
 // ------------------------------------------------------------------ B streamed past few rows of A
 
-constexpr int kI8StreamThreads = 6 * 32;  // producer, MMA, 4 epilogue warps
+constexpr int kI8StreamThreads = 7 * 32;  // B producer, MMA, 4 epilogue warps, A producer
 
-constexpr int kI8StreamScales = 256 * 4;  // token scales of the tile
+constexpr int kI8StreamScales = (256 + 128 + 128) * 4;  // token and channel scales, biases
 
 __host__ __device__ constexpr int i8_stream_stage_bytes(int bn) { return (128 + bn) * kI8BK; }
 constexpr int i8_stream_smem(int bn, int stages) {
     return kI8AlignSlack + stages * i8_stream_stage_bytes(bn) + kI8StreamScales + kI8BarrierBytes;
 }
 
-__device__ __forceinline__ int4 ld_cluster_v4(uint32_t addr) {
+template <bool kRemote>
+__device__ __forceinline__ int4 ld_sums(uint32_t addr) {
     int4 v;
-    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "r"(addr)
-                 : "memory");
+    if constexpr (kRemote)
+        asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "r"(addr));
+    else
+        asm volatile("ld.shared.v4.s32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "r"(addr));
     return v;
 }
 
@@ -472,6 +507,8 @@ __global__ void __launch_bounds__(kI8StreamThreads)
     const uint32_t stage_bytes = uint32_t(i8_stream_stage_bytes(bn));
     const uint32_t bars = base + stages * stage_bytes + kI8StreamScales;
     float* token_scale = reinterpret_cast<float*>(base_ptr + stages * stage_bytes);
+    float* channel_scale = token_scale + 256;
+    float* channel_bias = channel_scale + 128;
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (kI8MaxStages + s); };
     const uint32_t done_bar = bars + 8u * (2 * kI8MaxStages);
@@ -486,7 +523,25 @@ __global__ void __launch_bounds__(kI8StreamThreads)
     uint32_t tmem_cols = 32;
     while (int(tmem_cols) < bn) tmem_cols *= 2;
 
+    const int f0 = int(blockIdx.x / SPLIT) * 128;
+    const int t0 = int(blockIdx.y) * bn;
+    const int num_kb = (p.K + kI8BK - 1) / kI8BK;
+    const int kb0 = int((long long)num_kb * rank / SPLIT);
+    const int kb1 = int((long long)num_kb * (rank + 1) / SPLIT);
+    // K block of this CTA's i-th step, and the loads of a step.
+    const int turn = i8_first_block(3 * int(blockIdx.x / SPLIT) + 5 * int(blockIdx.y), kb1 - kb0);
+    auto block_of = [&](int i) {
+        const int kb = kb0 + turn + i;
+        return kb < kb1 ? kb : kb - (kb1 - kb0);
+    };
+    auto load_b = [&](int stage, int kb) {
+        mbar_arrive_expect_tx(full_bar(stage), stage_bytes);
+        tma_load_2d(base + stage * stage_bytes, &tmap_b, full_bar(stage), kb * kI8BK, f0);
+    };
+
+    if (threadIdx.x == 32 * 6) tma_prefetch_desc(&tmap_a);
     if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tmap_b);
         for (int s = 0; s < stages; ++s) {
             mbar_init(full_bar(s), 1);
             mbar_init(empty_bar(s), 1);
@@ -495,8 +550,9 @@ __global__ void __launch_bounds__(kI8StreamThreads)
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
         fence_barrier_init();
-        tma_prefetch_desc(&tmap_a);
-        tma_prefetch_desc(&tmap_b);
+        // The first stages of B, the bulk of the bytes, do not wait for the rest
+        // of the set-up.
+        for (int s = 0; s < min(stages, kb1 - kb0); ++s) load_b(s, block_of(s));
     }
     if (warp == 1) {
         tmem_alloc<1>(smem_u32(tmem_slot), tmem_cols);
@@ -507,77 +563,79 @@ __global__ void __launch_bounds__(kI8StreamThreads)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
-    const int f0 = int(blockIdx.x / SPLIT) * 128;
-    const int t0 = int(blockIdx.y) * bn;
-    const int num_kb = (p.K + kI8BK - 1) / kI8BK;
-    const int kb0 = int((long long)num_kb * rank / SPLIT);
-    const int kb1 = int((long long)num_kb * (rank + 1) / SPLIT);
     const int quad = warp & 3;
     const uint32_t lane_taddr = tmem_base + (uint32_t(quad * 32) << 16);
     const T* bias = static_cast<const T*>(p.bias);
     T* C = static_cast<T*>(p.C);
-    int ok = 1;
 
-    if (warp == 0 && lane == 0) {
-        int stage = 0;
-        uint32_t phase = 0;
-        int issued = 0;
+    if ((warp == 0 || warp == 6) && lane == 0) {
+        // Warp 0 loads B and arms the stage, warp 6 loads A. A load may complete
+        // before its phase is armed; the phase cannot finish before the arming
+        // thread arrives. B's first stages are under way already.
+        const bool loads_b = warp == 0;
+        const int first = loads_b ? min(stages, kb1 - kb0) : 0;
+        int stage = first == stages ? 0 : first;
+        uint32_t phase = first == stages ? 1u : 0u;
         bool live = true;
-        int kb = kb0 + i8_first_block(3 * int(blockIdx.x / SPLIT) + 5 * int(blockIdx.y), kb1 - kb0);
-        for (int i = kb0; i < kb1; ++i) {
+        for (int i = first; i < kb1 - kb0; ++i) {
             if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.err, kErrTimeoutProducer)) {
                 live = false;
                 break;
             }
-            const uint32_t sb = base + stage * stage_bytes;
-            mbar_arrive_expect_tx(full_bar(stage), stage_bytes);
-            tma_load_2d(sb, &tmap_b, full_bar(stage), kb * kI8BK, f0);
-            tma_load_2d(sb + 128 * kI8BK, &tmap_a, full_bar(stage), kb * kI8BK, t0);
-            if (++kb == kb1) kb = kb0;
-            ++issued;
+            if (loads_b)
+                load_b(stage, block_of(i));
+            else
+                tma_load_2d(base + stage * stage_bytes + 128 * kI8BK, &tmap_a, full_bar(stage),
+                            block_of(i) * kI8BK, t0);
             if (++stage == stages) {
                 stage = 0;
                 phase ^= 1u;
             }
         }
-        if (!live) {
-            for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
-                mbar_wait(full_bar(i % stages), uint32_t((i / stages) & 1), nullptr, p.err,
-                          kErrTimeoutDrain);
-        }
-    } else if (warp == 1 && lane == 0) {
+        if (!live) i8_let_loads_land();
+    } else if (warp == 1) {
         const uint32_t idesc = make_idesc_i8_s32(128, bn);
         int stage = 0;
         uint32_t phase = 0;
         bool live = true;
         for (int kb = kb0; kb < kb1; ++kb) {
-            if (!mbar_wait(full_bar(stage), phase, abort_flag, p.err, kErrTimeoutMma)) {
-                live = false;
-                break;
-            }
+            live = __all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, abort_flag, p.err,
+                                                     kErrTimeoutMma));
+            if (!live) break;
             tc_fence_after();
             const uint32_t sb = base + stage * stage_bytes;
-            const uint32_t sa = sb + 128 * kI8BK;
+            const uint64_t db = make_smem_desc<128>(sb);
+            const uint64_t da = make_smem_desc<128>(sb + 128 * kI8BK);
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < kI8BK / 32; ++kk)
-                umma_i8<1>(tmem_base, make_smem_desc<128>(sb + kk * 32),
-                           make_smem_desc<128>(sa + kk * 32), idesc,
-                           (kb > kb0 || kk > 0) ? 1u : 0u);
-            umma_commit(empty_bar(stage));
+                for (int kk = 0; kk < kI8BK / 32; ++kk)
+                    umma_i8<1>(tmem_base, db + 2 * kk, da + 2 * kk, idesc,
+                               (kb > kb0 || kk > 0) ? 1u : 0u);
+                umma_commit(empty_bar(stage));
+            }
+            __syncwarp();
             if (++stage == stages) {
                 stage = 0;
                 phase ^= 1u;
             }
         }
-        if (live) {
-            umma_commit(done_bar);
-        } else {
-            umma_commit(drain_bar);
-            mbar_wait(drain_bar, 0, nullptr, p.err, kErrTimeoutDrain);
+        if (elect_one()) {
+            if (live) {
+                umma_commit(done_bar);
+            } else {
+                umma_commit(drain_bar);
+                mbar_wait(drain_bar, 0, nullptr, p.err, kErrTimeoutDrain);
+            }
         }
-    } else if (warp >= 2) {
+    } else if (warp >= 2 && warp < 6) {
         for (int i = int(threadIdx.x) - 64; i < bn; i += 128)
             token_scale[i] = t0 + i < p.M ? p.sa[t0 + i] : 0.0f;
+        {
+            const int i = int(threadIdx.x) - 64;
+            channel_scale[i] = f0 + i < p.N ? p.sb[f0 + i] : 0.0f;
+            channel_bias[i] = bias && f0 + i < p.N ? OutType<T>::up(bias[f0 + i]) : 0.0f;
+        }
+        int ok = 1;
         if (lane == 0) ok = mbar_wait(done_bar, 0, abort_flag, p.err, kErrTimeoutEpilogue);
         ok = __shfl_sync(0xffffffffu, ok, 0);
         tc_fence_after();
@@ -594,35 +652,35 @@ __global__ void __launch_bounds__(kI8StreamThreads)
     }
 
     tc_fence_before();
+    __syncthreads();
+    // TMEM goes back before this CTA waits for its cluster. A rank may itself be
+    // waiting for TMEM, held by a CTA of another kernel that waits for TMEM held
+    // here (a pair of the FP16 family, launched on another stream).
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc<1>(tmem_base, tmem_cols);
+    }
     __syncwarp();
-    if constexpr (SPLIT > 1)
-        cluster_sync();  // every rank's sums are in its shared memory
-    else
-        __syncthreads();
-    if (warp >= 2 && ok) {
+    if constexpr (SPLIT > 1) cluster_sync();  // every rank's sums are in its shared memory
+    if (!*abort_flag) {
         // A warp takes whole tokens, four channels to a lane, so that the sums
         // are read and C is written in full lines; the tokens are dealt to the
-        // ranks and their warps in turn, four at a time in flight.
+        // ranks and their warps (all of them by now idle) in turn, several at a
+        // time in flight.
         const int f = f0 + lane * 4;
         const int in = p.N - f;  // channels of this lane inside C
-        float4 channel, b;
-        channel.x = in > 0 ? p.sb[f] : 0.0f;
-        channel.y = in > 1 ? p.sb[f + 1] : 0.0f;
-        channel.z = in > 2 ? p.sb[f + 2] : 0.0f;
-        channel.w = in > 3 ? p.sb[f + 3] : 0.0f;
-        b.x = bias && in > 0 ? OutType<T>::up(bias[f]) : 0.0f;
-        b.y = bias && in > 1 ? OutType<T>::up(bias[f + 1]) : 0.0f;
-        b.z = bias && in > 2 ? OutType<T>::up(bias[f + 2]) : 0.0f;
-        b.w = bias && in > 3 ? OutType<T>::up(bias[f + 3]) : 0.0f;
+        const float4 channel = *reinterpret_cast<const float4*>(channel_scale + lane * 4);
+        const float4 b = *reinterpret_cast<const float4*>(channel_bias + lane * 4);
         const int live = min(bn, p.M - t0);  // tokens of this tile
         uint32_t peer[SPLIT];
 #pragma unroll
         for (int s = 0; s < SPLIT; ++s)
             peer[s] = SPLIT > 1 ? map_to_cta(base + uint32_t(lane * 16), s)
                                 : base + uint32_t(lane * 16);
-        constexpr int kStep = 4 * SPLIT;  // tokens between two of one warp's
-        constexpr int kFlight = SPLIT >= 8 ? 2 : 4;
-        for (int t = rank + (warp - 2) * SPLIT; t < live; t += kFlight * kStep) {
+        constexpr int kStep = (kI8StreamThreads / 32) * SPLIT;  // tokens between two of a warp's
+        constexpr int kFlight = SPLIT >= 8 ? 2 : SPLIT >= 4 ? 4 : 8;
+        for (int t = rank + warp * SPLIT; t < live; t += kFlight * kStep) {
             int4 sum[kFlight];
 #pragma unroll
             for (int i = 0; i < kFlight; ++i) {
@@ -631,7 +689,7 @@ __global__ void __launch_bounds__(kI8StreamThreads)
                 if (ti < live) {
 #pragma unroll
                     for (int s = 0; s < SPLIT; ++s) {
-                        const int4 v = ld_cluster_v4(peer[s] + uint32_t(ti) * 512u);
+                        const int4 v = ld_sums<(SPLIT > 1)>(peer[s] + uint32_t(ti) * 512u);
                         sum[i].x += v.x;
                         sum[i].y += v.y;
                         sum[i].z += v.z;
@@ -656,13 +714,6 @@ __global__ void __launch_bounds__(kI8StreamThreads)
     if constexpr (SPLIT > 1) {
         __syncwarp();
         cluster_sync();  // no rank leaves while another reads its sums
-    } else {
-        __syncthreads();
-    }
-    if (warp == 1) {
-        __syncwarp();
-        tc_fence_after();
-        tmem_dealloc<1>(tmem_base, tmem_cols);
     }
 }
 

@@ -125,6 +125,18 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
 }
 
+// One lane of a converged warp (the same one each time). Unlike a test of the
+// lane number it leaves the code around it warp-uniform for the compiler.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(yes));
+    return yes != 0;
+}
+
 // ---------------------------------------------------------------- cluster
 
 __device__ __forceinline__ uint32_t cluster_cta_rank() {
