@@ -41,18 +41,18 @@ def _type_code(dtype, what):
 
 def _rows(t, what):
     """(M, D, pitch) of a 2-D CUDA tensor with contiguous rows."""
-    if t.dim() != 2:
-        raise ValueError("%s is a matrix of rows, got shape %s" % (what, tuple(t.shape)))
+    shape = t.shape
+    if len(shape) != 2:
+        raise ValueError("%s is a matrix of rows, got shape %s" % (what, tuple(shape)))
     if not t.is_cuda:
         raise ValueError("%s is not a CUDA tensor" % what)
-    M, D = t.shape
-    if D > 1 and t.stride(1) != 1:
+    M, D = shape
+    pitch, step = t.stride()
+    if step != 1 and D > 1:
         raise ValueError("%s: rows must be contiguous (inner stride 1)" % what)
-    pitch = t.stride(0)
-    if M > 1:
-        if pitch < D:
+    if pitch < D:
+        if M > 1:
             raise ValueError("%s: rows overlap (pitch %d, length %d)" % (what, pitch, D))
-    elif pitch < D:
         pitch = D
     return M, D, pitch
 
@@ -73,56 +73,50 @@ def _vector(t, what, device, dtype, n):
         raise ValueError("%s must be contiguous" % what)
 
 
-class _Launch:
-    """The device and stream of one call: makes the tensors' device current and,
-    for a stream other than torch's current one, allocates from its pool."""
-
-    __slots__ = ("handle", "_contexts")
-
-    def __init__(self, device, stream):
-        import torch
-        index = device.index
-        self._contexts = ()
-        if index != torch.cuda.current_device():
-            self._contexts = (torch.cuda.device(index),)
+def _run(device, stream, call):
+    """call(handle) with the tensors' device current; on a stream other than torch's
+    current one, inside that stream's context, so that outputs come from its pool."""
+    import torch
+    index = device.index
+    if stream is None and torch._C._cuda_getDevice() == index:
+        return call(torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
         if stream is None:
-            self.handle = torch._C._cuda_getCurrentRawStream(index)
-            return
-        self.handle = stream if isinstance(stream, int) else stream.cuda_stream
-        if self.handle != torch._C._cuda_getCurrentRawStream(index):
-            if self.handle == 0:
-                s = torch.cuda.default_stream(index)
-            elif isinstance(stream, int):
-                s = torch.cuda.ExternalStream(stream, device=index)
-            else:
-                s = stream
-            self._contexts += (torch.cuda.stream(s),)
+            return call(torch._C._cuda_getCurrentRawStream(index))
+        handle = stream if isinstance(stream, int) else stream.cuda_stream
+        if handle == 0:
+            stream = torch.cuda.default_stream(index)
+        elif isinstance(stream, int):
+            stream = torch.cuda.ExternalStream(stream, device=index)
+        with torch.cuda.stream(stream):
+            return call(handle)
 
-    def __enter__(self):
-        for c in self._contexts:
-            c.__enter__()
-        return self.handle
 
-    def __exit__(self, *exc):
-        for c in reversed(self._contexts):
-            c.__exit__(*exc)
+def _new(shape, strides, dtype, device):
+    import torch
+    return torch.empty_strided(shape, strides, dtype=dtype, device=device)
+
+
+def _given(M, D, device, out, scale):
+    """Checks the arrays that a caller passed for (q, scale)."""
+    import torch
+    if out is not None:
+        _like(out, "out", device, torch.int8, (M, D))
+        _rows(out, "out")
+    if scale is not None:
+        _vector(scale, "scale", device, torch.float32, M)
 
 
 def _outputs(M, D, device, out, scale):
-    """(q, q's pitch, scale): the given arrays, checked, or new ones."""
+    """(q, q's pitch, scale): the given arrays or new ones."""
     import torch
     if out is None:
         pitch = (D + 15) // 16 * 16
-        out = torch.empty((M, pitch), dtype=torch.int8, device=device)
-        if pitch != D:
-            out = out[:, :D]
+        out = _new((M, D), (pitch, 1), torch.int8, device)
     else:
-        _like(out, "out", device, torch.int8, (M, D))
-        pitch = _rows(out, "out")[2]
+        pitch = max(out.stride(0), D)
     if scale is None:
-        scale = torch.empty(M, dtype=torch.float32, device=device)
-    else:
-        _vector(scale, "scale", device, torch.float32, M)
+        scale = _new((M,), (1,), torch.float32, device)
     return out, pitch, scale
 
 
@@ -133,11 +127,17 @@ def quantize_i8(x, out=None, scale=None, stream=None):
     finite, and q = 0."""
     code = _type_code(x.dtype, "x")
     M, D, ldx = _rows(x, "x")
-    with _Launch(x.device, stream) as handle:
-        q, ldq, scale = _outputs(M, D, x.device, out, scale)
-        check(lib.ridge_quantize_i8(x.data_ptr(), code, q.data_ptr(), scale.data_ptr(), M, D, ldx,
-                                    ldq, handle), "ridge_quantize_i8 %dx%d" % (M, D))
-    return q, scale
+    device = x.device
+    _given(M, D, device, out, scale)
+
+    def call(handle):
+        q, ldq, s = _outputs(M, D, device, out, scale)
+        st = lib.ridge_quantize_i8(x.data_ptr(), code, q.data_ptr(), s.data_ptr(), M, D, ldx, ldq,
+                                   handle)
+        if st:
+            check(st, "ridge_quantize_i8 %dx%d" % (M, D))
+        return q, s
+    return _run(device, stream, call)
 
 
 def rms_norm_i8(x, weight, residual=None, eps=1e-6, out=None, scale=None, residual_out=None,
@@ -148,34 +148,39 @@ def rms_norm_i8(x, weight, residual=None, eps=1e-6, out=None, scale=None, residu
     x, residual (M, D) and weight (D,) have one type. h is rounded once to that type;
     the norm reads the unrounded sum. residual_out receives h and may be residual
     or x itself; by default it is a new tensor."""
-    import torch
     code = _type_code(x.dtype, "x")
     M, D, ldx = _rows(x, "x")
-    _vector(weight, "weight", x.device, x.dtype, D)
+    device, dtype = x.device, x.dtype
+    _vector(weight, "weight", device, dtype, D)
     eps = float(eps)
-    if not (eps > 0 and math.isfinite(eps)):
+    if not 0 < eps < math.inf:
         raise ValueError("eps is finite and above 0, got %r" % eps)
-    if residual is None and residual_out is not None:
-        raise ValueError("residual_out needs a residual")
     ldr = ldh = D
     if residual is not None:
-        _like(residual, "residual", x.device, x.dtype, x.shape)
+        _like(residual, "residual", device, dtype, x.shape)
         ldr = _rows(residual, "residual")[2]
         if residual_out is not None:
-            _like(residual_out, "residual_out", x.device, x.dtype, x.shape)
+            _like(residual_out, "residual_out", device, dtype, x.shape)
             ldh = _rows(residual_out, "residual_out")[2]
-    with _Launch(x.device, stream) as handle:
-        q, ldq, scale = _outputs(M, D, x.device, out, scale)
-        if residual is not None and residual_out is None:
-            residual_out = torch.empty((M, D), dtype=x.dtype, device=x.device)
-        # An empty tensor's address is null, which at the C ABI means "not given".
-        given = residual is not None and M > 0 and D > 0
-        check(lib.ridge_rms_norm_i8(x.data_ptr(), residual.data_ptr() if given else None,
-                                    weight.data_ptr(), code,
-                                    residual_out.data_ptr() if given else None, q.data_ptr(),
-                                    scale.data_ptr(), M, D, ldx, ldr, ldh, ldq, eps, handle),
-              "ridge_rms_norm_i8 %dx%d" % (M, D))
-    return q, scale, residual_out
+    elif residual_out is not None:
+        raise ValueError("residual_out needs a residual")
+    _given(M, D, device, out, scale)
+    # An empty tensor's address is null, which at the C ABI means "not given".
+    add = residual is not None and M > 0 and D > 0
+
+    def call(handle):
+        q, ldq, s = _outputs(M, D, device, out, scale)
+        h = residual_out
+        if h is None and residual is not None:
+            h = _new((M, D), (D, 1), dtype, device)
+        st = lib.ridge_rms_norm_i8(x.data_ptr(), residual.data_ptr() if add else None,
+                                   weight.data_ptr(), code, h.data_ptr() if add else None,
+                                   q.data_ptr(), s.data_ptr(), M, D, ldx, ldr, ldh, ldq, eps,
+                                   handle)
+        if st:
+            check(st, "ridge_rms_norm_i8 %dx%d" % (M, D))
+        return q, s, h
+    return _run(device, stream, call)
 
 
 def silu_mul_i8(gate, up, out=None, scale=None, stream=None):
@@ -183,14 +188,19 @@ def silu_mul_i8(gate, up, out=None, scale=None, stream=None):
     type and may be the two halves of one (M, 2 D) tensor."""
     code = _type_code(gate.dtype, "gate")
     M, D, ldg = _rows(gate, "gate")
-    _like(up, "up", gate.device, gate.dtype, gate.shape)
+    device = gate.device
+    _like(up, "up", device, gate.dtype, gate.shape)
     ldu = _rows(up, "up")[2]
-    with _Launch(gate.device, stream) as handle:
-        q, ldq, scale = _outputs(M, D, gate.device, out, scale)
-        check(lib.ridge_silu_mul_i8(gate.data_ptr(), up.data_ptr(), code, q.data_ptr(),
-                                    scale.data_ptr(), M, D, ldg, ldu, ldq, handle),
-              "ridge_silu_mul_i8 %dx%d" % (M, D))
-    return q, scale
+    _given(M, D, device, out, scale)
+
+    def call(handle):
+        q, ldq, s = _outputs(M, D, device, out, scale)
+        st = lib.ridge_silu_mul_i8(gate.data_ptr(), up.data_ptr(), code, q.data_ptr(),
+                                   s.data_ptr(), M, D, ldg, ldu, ldq, handle)
+        if st:
+            check(st, "ridge_silu_mul_i8 %dx%d" % (M, D))
+        return q, s
+    return _run(device, stream, call)
 
 
 def dequantize_i8(q, scale, out=None, dtype=None, stream=None):
@@ -204,16 +214,20 @@ def dequantize_i8(q, scale, out=None, dtype=None, stream=None):
     if dtype is None:
         dtype = torch.float16 if out is None else out.dtype
     code = _type_code(dtype, "dtype")
+    device = q.device
     ldo = D
     if out is not None:
-        _like(out, "out", q.device, dtype, q.shape)
+        _like(out, "out", device, dtype, q.shape)
         ldo = _rows(out, "out")[2]
-    with _Launch(q.device, stream) as handle:
-        if out is None:
-            out = torch.empty((M, D), dtype=dtype, device=q.device)
-        check(lib.ridge_dequantize_i8(q.data_ptr(), scale.data_ptr(), code, out.data_ptr(), M, D,
-                                      ldq, ldo, handle), "ridge_dequantize_i8 %dx%d" % (M, D))
-    return out
+
+    def call(handle):
+        o = _new((M, D), (D, 1), dtype, device) if out is None else out
+        st = lib.ridge_dequantize_i8(q.data_ptr(), scale.data_ptr(), code, o.data_ptr(), M, D,
+                                     ldq, ldo, handle)
+        if st:
+            check(st, "ridge_dequantize_i8 %dx%d" % (M, D))
+        return o
+    return _run(device, stream, call)
 
 
 def gemm_i8(a, a_scale, b, b_scale, bias=None, out=None, dtype=None, stream=None):
@@ -231,24 +245,27 @@ def gemm_i8(a, a_scale, b, b_scale, bias=None, out=None, dtype=None, stream=None
     if K != Kb:
         raise ValueError("expected a (M, K) and b (N, K), got %s and %s" % (tuple(a.shape),
                                                                          tuple(b.shape)))
-    if b.device != a.device:
-        raise ValueError("b is on %s, expected %s" % (b.device, a.device))
-    _vector(a_scale, "a_scale", a.device, torch.float32, M)
-    _vector(b_scale, "b_scale", a.device, torch.float32, N)
+    device = a.device
+    if b.device != device:
+        raise ValueError("b is on %s, expected %s" % (b.device, device))
+    _vector(a_scale, "a_scale", device, torch.float32, M)
+    _vector(b_scale, "b_scale", device, torch.float32, N)
     if dtype is None:
         dtype = torch.float16 if out is None else out.dtype
     code = _type_code(dtype, "dtype")
     if bias is not None:
-        _vector(bias, "bias", a.device, dtype, N)
+        _vector(bias, "bias", device, dtype, N)
     ldc = N
     if out is not None:
-        _like(out, "out", a.device, dtype, (M, N))
+        _like(out, "out", device, dtype, (M, N))
         ldc = _rows(out, "out")[2]
-    with _Launch(a.device, stream) as handle:
-        if out is None:
-            out = torch.empty((M, N), dtype=dtype, device=a.device)
-        check(lib.ridge_gemm_i8(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(),
-                                b_scale.data_ptr(), None if bias is None else bias.data_ptr(),
-                                code, out.data_ptr(), M, N, K, lda, ldb, ldc, handle),
-              "ridge_gemm_i8 %dx%dx%d" % (M, N, K))
-    return out
+
+    def call(handle):
+        o = _new((M, N), (N, 1), dtype, device) if out is None else out
+        st = lib.ridge_gemm_i8(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(),
+                               None if bias is None else bias.data_ptr(), code, o.data_ptr(), M, N,
+                               K, lda, ldb, ldc, handle)
+        if st:
+            check(st, "ridge_gemm_i8 %dx%dx%d" % (M, N, K))
+        return o
+    return _run(device, stream, call)
