@@ -39,6 +39,7 @@ __global__ void ridge_gemm_i8_empty(const I8Params p) {
 struct Plan {
     bool stream;
     int bn, stages;
+    int sub;          // stream: K blocks to a stage
     int split;        // stream: CTAs of a cluster that share K
     int64_t items;    // units of work: tiles and strips, or CTAs of the streaming kernel
     int whole, cut;   // tile: see I8Params
@@ -69,10 +70,10 @@ Plan tile_plan(int64_t M, int64_t N, int bn, int pairs) {
 }
 
 // CTAs of the streaming kernel that share an SM with this ring.
-int stream_residents(int bn, int stages) {
+int stream_residents(int bn, int blocks) {
     int cols = 32;
     while (cols < bn) cols *= 2;
-    const int by_smem = kSmemPerSm / (i8_stream_smem(bn, stages) + kSmemReservedPerCta);
+    const int by_smem = kSmemPerSm / (i8_stream_smem(bn, blocks) + kSmemReservedPerCta);
     return std::max(1, std::min(by_smem, kTmemColsPerSm / cols));
 }
 
@@ -86,11 +87,16 @@ Plan stream_plan(int64_t M, int64_t N, int bn, int split, int num_sms) {
     const int64_t token_tiles = ceil_div(M, bn);
     p.bn = int(ceil_div(ceil_div(M, token_tiles), 16) * 16);
     p.items = ceil_div(N, 128) * ceil_div(M, p.bn) * split;
-    const int fixed = i8_stream_smem(p.bn, 0), stage = i8_stream_stage_bytes(p.bn);
+    // Two K blocks to a stage halve the barrier waits a block costs (1 x 1024 x
+    // 4096 5.6 -> 5.2 us, 16 x 11008 x 512 4.8 -> 4.3); from 128 tokens on the ring
+    // has too few stages left for it (128 x 8192 x 8192 19.2 -> 19.6).
+    p.sub = p.bn <= 64 ? 2 : 1;
+    const int fixed = i8_stream_smem(p.bn, 0);
+    const int stage = p.sub * i8_stream_block_bytes(p.bn);
     p.stages = stages_for(stage, fixed, kMaxDynSmem);
     if (p.items > num_sms) {
         const int half = stages_for(stage, fixed, kSmemPerSm / 2 - kSmemReservedPerCta);
-        if (half >= 3) p.stages = half;
+        if (half * p.sub >= 3) p.stages = half;
     }
     return p;
 }
@@ -100,29 +106,32 @@ Plan stream_plan(int64_t M, int64_t N, int bn, int split, int num_sms) {
 // and ring below). The plan they pick is on average 1.5% slower than the best of a
 // shape, 12% at worst.
 //
-// A streaming CTA takes 0.26 us for a K block of its own and an SM takes in
+// A streaming CTA takes 0.26 us for a K block of its own (0.23 with two to a
+// stage) and an SM takes in
 // 97 bytes/ns for all of its CTAs; sums leave at 20 ns a token, over a cluster
 // with 1 us + 70 ns a rank for the exchange. Clusters of 4 and 8 do not find
 // room on every SM.
 double stream_time(const Plan& p, int64_t num_kb, int num_sms) {
     const double room = p.split == 8 ? 0.757 : p.split == 4 ? 0.892 : 1.0;
     const int64_t at_once = std::max<int64_t>(
-        1, int64_t(stream_residents(p.bn, p.stages) * room * num_sms));
+        1, int64_t(stream_residents(p.bn, p.stages * p.sub) * room * num_sms));
     const int64_t waves = ceil_div(p.items, at_once);
     const int64_t per_sm = std::max(waves, ceil_div(p.items, num_sms));
     const double steps = double(ceil_div(num_kb, p.split));
     const double out = (p.split > 1 ? 1.0 + 0.07 * p.split : 0.25) + 0.02 * p.bn;
-    const double feed = i8_stream_stage_bytes(p.bn) / 97e3;
-    return 4.2 + waves * out + steps * std::max(0.26 * waves, feed * per_sm);
+    const double feed = i8_stream_block_bytes(p.bn) / 97e3;
+    return 4.2 + waves * out + steps * std::max((p.sub == 2 ? 0.23 : 0.26) * waves, feed * per_sm);
 }
 
-// A pair takes 0.35 to 0.38 us for a K block, little less for narrow tiles.
+// A pair takes 0.35 to 0.38 us for a K block, little less for narrow tiles, and
+// 2.4 us to drain 256 columns, which bounds a tile of few K blocks.
 double tile_time(const Plan& p, int64_t num_kb, int pairs) {
-    auto step = [](int width) { return width == 256 ? 0.38 : width == 192 ? 0.36 : 0.35; };
+    auto round = [&](int width) {
+        const double block = width == 256 ? 0.38 : width == 192 ? 0.36 : 0.35;
+        return std::max(block * num_kb, 2.4 * width / 256);
+    };
     const int64_t rounds = p.cut > 1 ? p.whole / pairs : ceil_div(p.items, pairs);
-    double t = 7.4 + double(rounds) * num_kb * step(p.bn);
-    if (p.cut > 1) t += num_kb * step(p.bn / p.cut);
-    return t;
+    return 7.4 + rounds * round(p.bn) + (p.cut > 1 ? round(p.bn / p.cut) : 0.0);
 }
 
 // The kernel and tile with the least estimated time. Sums are exact integers, so
@@ -130,10 +139,11 @@ double tile_time(const Plan& p, int64_t num_kb, int pairs) {
 Plan make_plan(int64_t M, int64_t N, int64_t K, int num_sms, int pairs) {
 #ifdef RIDGE_I8_PROBE
     if (const char* v = std::getenv("RIDGE_I8_PLAN")) {
-        int s = 0, bn = 0, stages = 0, split = 0;
-        std::sscanf(v, "%d,%d,%d,%d", &s, &bn, &stages, &split);
+        int s = 0, bn = 0, stages = 0, split = 0, sub = 1;
+        std::sscanf(v, "%d,%d,%d,%d,%d", &s, &bn, &stages, &split, &sub);
         Plan p = s ? stream_plan(M, N, bn, split, num_sms) : tile_plan(M, N, bn, pairs);
         p.stages = stages;
+        p.sub = sub;
         return p;
     }
 #endif
@@ -250,7 +260,7 @@ int launch_stream(const Plan& plan, const CUtensorMap& a, const CUtensorMap& b,
     cfg.gridDim = dim3(unsigned(ceil_div(p.N, 128) * SPLIT), unsigned(ceil_div(p.M, plan.bn)));
     if (cfg.gridDim.y > 65535) return RIDGE_EINVAL;
     cfg.blockDim = dim3(kI8StreamThreads);
-    cfg.dynamicSmemBytes = size_t(i8_stream_smem(plan.bn, plan.stages));
+    cfg.dynamicSmemBytes = size_t(i8_stream_smem(plan.bn, plan.stages * plan.sub));
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     if (SPLIT > 1) set_cluster(&cfg, attr, SPLIT);
@@ -273,6 +283,7 @@ int run_product(const int8_t* A, const int8_t* B, int32_t type, int64_t lda, int
     const Plan plan = make_plan(p.M, p.N, p.K, dev.num_sms, pairs);
     p.bn = plan.bn;
     p.stages = plan.stages;
+    p.sub = plan.sub;
     CUtensorMap a, b;
     st = operand_map(&a, A, p.M, p.K, lda, plan.stream ? plan.bn : 128);
     if (st != RIDGE_OK) return st;
@@ -323,8 +334,8 @@ extern "C" int ridge_gemm_i8(const int8_t* A, const float* scale_a, const int8_t
                              int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb,
                              int64_t ldc, void* stream_v) {
     const int size = type_size(type);
-    const int64_t kExtent = int64_t(1) << 31;
-    if (size == 0 || M < 0 || N < 0 || K < 0 || M >= kExtent || N >= kExtent) return RIDGE_EINVAL;
+    const int64_t kExtent = int64_t(1) << 30;  // a tile past the last row still has 32-bit indices
+    if (size == 0 || M < 0 || N < 0 || K < 0 || M > kExtent || N > kExtent) return RIDGE_EINVAL;
     if (K >= int64_t(1) << 17) return RIDGE_EINVAL;  // 2^17 products of 2^14 could overflow
     // One row has no pitch of its own: any that the tensor map takes will do.
     const int64_t whole = (std::max<int64_t>(K, 1) + 15) / 16 * 16;

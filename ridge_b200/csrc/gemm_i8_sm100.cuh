@@ -55,6 +55,7 @@ struct I8Params {
     int whole;      // tile: tiles computed bn wide; each later one is cut into `cut` narrower
     int cut;        // ones (1, 2 or 4, widths of whole 64s) that fill the last round
     int stages;
+    int sub;        // stream: K blocks to a ring stage (1 or 2)
     int groupM;
     int tma_store;  // tile: C is stored through its tensor map; 0: from shared memory by threads
     int vec_store;  // stream: rows of C start on four elements
@@ -454,9 +455,9 @@ constexpr int kI8StreamThreads = 7 * 32;  // B producer, MMA, 4 epilogue warps, 
 
 constexpr int kI8StreamScales = (256 + 128 + 128) * 4;  // token and channel scales, biases
 
-__host__ __device__ constexpr int i8_stream_stage_bytes(int bn) { return (128 + bn) * kI8BK; }
-constexpr int i8_stream_smem(int bn, int stages) {
-    return kI8AlignSlack + stages * i8_stream_stage_bytes(bn) + kI8StreamScales + kI8BarrierBytes;
+__host__ __device__ constexpr int i8_stream_block_bytes(int bn) { return (128 + bn) * kI8BK; }
+constexpr int i8_stream_smem(int bn, int blocks) {
+    return kI8AlignSlack + blocks * i8_stream_block_bytes(bn) + kI8StreamScales + kI8BarrierBytes;
 }
 
 template <bool kRemote>
@@ -504,7 +505,9 @@ __global__ void __launch_bounds__(kI8StreamThreads)
 
     const int stages = p.stages;
     const int bn = p.bn;
-    const uint32_t stage_bytes = uint32_t(i8_stream_stage_bytes(bn));
+    const int sub = p.sub;
+    const uint32_t block_bytes = uint32_t(i8_stream_block_bytes(bn));
+    const uint32_t stage_bytes = uint32_t(sub) * block_bytes;
     const uint32_t bars = base + stages * stage_bytes + kI8StreamScales;
     float* token_scale = reinterpret_cast<float*>(base_ptr + stages * stage_bytes);
     float* channel_scale = token_scale + 256;
@@ -528,15 +531,26 @@ __global__ void __launch_bounds__(kI8StreamThreads)
     const int num_kb = (p.K + kI8BK - 1) / kI8BK;
     const int kb0 = int((long long)num_kb * rank / SPLIT);
     const int kb1 = int((long long)num_kb * (rank + 1) / SPLIT);
-    // K block of this CTA's i-th step, and the loads of a step.
-    const int turn = i8_first_block(3 * int(blockIdx.x / SPLIT) + 5 * int(blockIdx.y), kb1 - kb0);
+    const int blocks = kb1 - kb0;
+    const int steps = (blocks + sub - 1) / sub;
+    // K block of this CTA's i-th place, and the loads of a step: B arms the stage.
+    const int turn = i8_first_block(3 * int(blockIdx.x / SPLIT) + 5 * int(blockIdx.y), blocks);
     auto block_of = [&](int i) {
         const int kb = kb0 + turn + i;
-        return kb < kb1 ? kb : kb - (kb1 - kb0);
+        return kb < kb1 ? kb : kb - blocks;
     };
-    auto load_b = [&](int stage, int kb) {
-        mbar_arrive_expect_tx(full_bar(stage), stage_bytes);
-        tma_load_2d(base + stage * stage_bytes, &tmap_b, full_bar(stage), kb * kI8BK, f0);
+    auto load_b = [&](int stage, int step) {
+        const int n = min(sub, blocks - step * sub);
+        mbar_arrive_expect_tx(full_bar(stage), uint32_t(n) * block_bytes);
+        for (int j = 0; j < n; ++j)
+            tma_load_2d(base + stage * stage_bytes + j * block_bytes, &tmap_b, full_bar(stage),
+                        block_of(step * sub + j) * kI8BK, f0);
+    };
+    auto load_a = [&](int stage, int step) {
+        const int n = min(sub, blocks - step * sub);
+        for (int j = 0; j < n; ++j)
+            tma_load_2d(base + stage * stage_bytes + j * block_bytes + 128 * kI8BK, &tmap_a,
+                        full_bar(stage), block_of(step * sub + j) * kI8BK, t0);
     };
 
     if (threadIdx.x == 32 * 6) tma_prefetch_desc(&tmap_a);
@@ -552,7 +566,7 @@ __global__ void __launch_bounds__(kI8StreamThreads)
         fence_barrier_init();
         // The first stages of B, the bulk of the bytes, do not wait for the rest
         // of the set-up.
-        for (int s = 0; s < min(stages, kb1 - kb0); ++s) load_b(s, block_of(s));
+        for (int s = 0; s < min(stages, steps); ++s) load_b(s, s);
     }
     if (warp == 1) {
         tmem_alloc<1>(smem_u32(tmem_slot), tmem_cols);
@@ -573,20 +587,19 @@ __global__ void __launch_bounds__(kI8StreamThreads)
         // before its phase is armed; the phase cannot finish before the arming
         // thread arrives. B's first stages are under way already.
         const bool loads_b = warp == 0;
-        const int first = loads_b ? min(stages, kb1 - kb0) : 0;
+        const int first = loads_b ? min(stages, steps) : 0;
         int stage = first == stages ? 0 : first;
         uint32_t phase = first == stages ? 1u : 0u;
         bool live = true;
-        for (int i = first; i < kb1 - kb0; ++i) {
+        for (int i = first; i < steps; ++i) {
             if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.err, kErrTimeoutProducer)) {
                 live = false;
                 break;
             }
             if (loads_b)
-                load_b(stage, block_of(i));
+                load_b(stage, i);
             else
-                tma_load_2d(base + stage * stage_bytes + 128 * kI8BK, &tmap_a, full_bar(stage),
-                            block_of(i) * kI8BK, t0);
+                load_a(stage, i);
             if (++stage == stages) {
                 stage = 0;
                 phase ^= 1u;
@@ -598,19 +611,22 @@ __global__ void __launch_bounds__(kI8StreamThreads)
         int stage = 0;
         uint32_t phase = 0;
         bool live = true;
-        for (int kb = kb0; kb < kb1; ++kb) {
+        for (int i = 0; i < steps; ++i) {
             live = __all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, abort_flag, p.err,
                                                      kErrTimeoutMma));
             if (!live) break;
             tc_fence_after();
             const uint32_t sb = base + stage * stage_bytes;
-            const uint64_t db = make_smem_desc<128>(sb);
-            const uint64_t da = make_smem_desc<128>(sb + 128 * kI8BK);
+            const int n = min(sub, blocks - i * sub);
             if (elect_one()) {
+                for (int j = 0; j < n; ++j) {
+                    const uint64_t db = make_smem_desc<128>(sb + j * block_bytes);
+                    const uint64_t da = make_smem_desc<128>(sb + j * block_bytes + 128 * kI8BK);
 #pragma unroll
-                for (int kk = 0; kk < kI8BK / 32; ++kk)
-                    umma_i8<1>(tmem_base, db + 2 * kk, da + 2 * kk, idesc,
-                               (kb > kb0 || kk > 0) ? 1u : 0u);
+                    for (int kk = 0; kk < kI8BK / 32; ++kk)
+                        umma_i8<1>(tmem_base, db + 2 * kk, da + 2 * kk, idesc,
+                                   (i > 0 || j > 0 || kk > 0) ? 1u : 0u);
+                }
                 umma_commit(empty_bar(stage));
             }
             __syncwarp();

@@ -35,6 +35,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace ridge_b200 {
 
@@ -56,6 +57,7 @@ struct RowParams {
 template <typename T>
 constexpr int kVecOf = 16 / int(sizeof(T));
 
+// One element, or the two 16-bit elements of a 32-bit word.
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -69,17 +71,59 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
     return __float2bfloat16_rn(v);
 }
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
 
 // VEC elements as they lie in memory: one 16-byte load, or a single element
 // where the row's start or length is no multiple of 16 bytes.
 template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) Chunk {
-    T e[VEC];
-};
+    static constexpr bool kPairs = sizeof(T) == 2 && VEC > 1;
+    using Raw = typename std::conditional<kPairs, uint32_t, T>::type;
+    static constexpr int kRaw = kPairs ? VEC / 2 : VEC;
+    Raw raw[kRaw];
 
-template <int VEC>
-struct alignas(VEC) Bytes {
-    int8_t b[VEC];
+    __device__ __forceinline__ void get(float (&f)[VEC]) const {
+#pragma unroll
+        for (int i = 0; i < kRaw; ++i) {
+            if constexpr (kPairs) {
+                const float2 v = unpack2<T>(raw[i]);
+                f[2 * i] = v.x;
+                f[2 * i + 1] = v.y;
+            } else {
+                f[i] = to_f32(raw[i]);
+            }
+        }
+    }
+    __device__ __forceinline__ void set(const float (&f)[VEC]) {
+#pragma unroll
+        for (int i = 0; i < kRaw; ++i) {
+            if constexpr (kPairs)
+                raw[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
+            else
+                raw[i] = from_f32<T>(f[i]);
+        }
+    }
 };
 
 // Low bytes of the rounded sums v * inv + 1.5 * 2^23, four to a word.
@@ -88,19 +132,18 @@ __device__ __forceinline__ uint32_t round_bits(float v, float inv) {
 }
 
 template <int VEC>
-__device__ __forceinline__ void store_q(int8_t* dst, const float (&v)[VEC], float pre, float inv,
-                                        bool zero) {
+__device__ __forceinline__ void store_q(int8_t* dst, const float (&v)[VEC], float inv, bool zero) {
     if constexpr (VEC == 1) {
-        const uint32_t b = round_bits(v[0] * pre, inv);
+        const uint32_t b = round_bits(v[0], inv);
         *dst = zero ? int8_t(0) : int8_t(b & 0xffu);
     } else {
         uint32_t word[VEC / 4];
 #pragma unroll
         for (int i = 0; i < VEC / 4; ++i) {
-            const uint32_t lo = __byte_perm(round_bits(v[4 * i] * pre, inv),
-                                            round_bits(v[4 * i + 1] * pre, inv), 0x0040);
-            const uint32_t hi = __byte_perm(round_bits(v[4 * i + 2] * pre, inv),
-                                            round_bits(v[4 * i + 3] * pre, inv), 0x0040);
+            const uint32_t lo = __byte_perm(round_bits(v[4 * i], inv),
+                                            round_bits(v[4 * i + 1], inv), 0x0040);
+            const uint32_t hi = __byte_perm(round_bits(v[4 * i + 2], inv),
+                                            round_bits(v[4 * i + 3], inv), 0x0040);
             word[i] = zero ? 0u : __byte_perm(lo, hi, 0x5410);
         }
         if constexpr (VEC == 8)
@@ -110,32 +153,56 @@ __device__ __forceinline__ void store_q(int8_t* dst, const float (&v)[VEC], floa
     }
 }
 
+// max(|a|, |b|, |c|), NaN if any is.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+    float m;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+    return m;
+}
+
+// x / (1 + e^-x), with one ex2 and one reciprocal of the hardware's (each within
+// 2^-22.5 relative; the exponent's rounding adds |x| 2^-23.4 to e^-x, which reaches
+// the result times e^-x / (1 + e^-x)). e^-x = inf gives -0 for finite x, and NaN
+// for x = -inf, as the formula does.
+__device__ __forceinline__ float silu(float x) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return x * r;
+}
+
 // v and, for kNormAdd, the stored sum of one chunk; adds to the row's sum of
-// squares and raises the row's maximum of |v|. The maximum is kept on the bits
-// of |v|, whose order as unsigned numbers is that of the values with every NaN
-// above infinity, so a NaN is never dropped.
+// squares and raises the row's maximum of |v|, which keeps a NaN.
 template <typename T, int OP, int VEC>
 __device__ __forceinline__ void take_chunk(const Chunk<T, VEC>& x, const Chunk<T, VEC>& r,
                                            const Chunk<T, VEC>& w, Chunk<T, VEC>& h,
-                                           float (&v)[VEC], float& sumsq, uint32_t& top) {
+                                           float (&v)[VEC], float& sumsq, float& top) {
+    float other[VEC];
+    x.get(v);
+    if constexpr (OP == kNormAdd) {
+        r.get(other);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        float a = to_f32(x.e[i]);
-        if constexpr (OP == kNormAdd) {
-            a += to_f32(r.e[i]);
-            h.e[i] = from_f32<T>(a);
+        for (int i = 0; i < VEC; ++i) v[i] += other[i];
+        h.set(v);
+    }
+    if constexpr (OP == kNorm || OP == kNormAdd) {
+        w.get(other);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            sumsq = fmaf(v[i], v[i], sumsq);
+            v[i] *= other[i];
         }
-        if constexpr (OP == kNorm || OP == kNormAdd) {
-            sumsq = fmaf(a, a, sumsq);
-            a *= to_f32(w.e[i]);
-        }
-        if constexpr (OP == kSiluMul) {
-            // __expf is off by 2^-22 + |x| 2^-24 relative; for x > 0 that reaches y
-            // times e^-x, and for x << 0 y itself is small beside the row's maximum.
-            a = __fdividef(a, 1.0f + __expf(-a)) * to_f32(r.e[i]);
-        }
-        v[i] = a;
-        top = max(top, __float_as_uint(a) & 0x7fffffffu);
+    }
+    if constexpr (OP == kSiluMul) {
+        r.get(other);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = silu(v[i]) * other[i];
+    }
+    if constexpr (VEC == 1) {
+        top = max_abs(top, v[0], v[0]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) top = max_abs(top, v[i], v[i + 1]);
     }
 }
 
@@ -146,28 +213,38 @@ struct RowScale {
 };
 
 template <int OP>
-__device__ __forceinline__ RowScale row_scale(float sumsq, uint32_t top, int D, float eps) {
-    const float amax = __uint_as_float(top);
+__device__ __forceinline__ RowScale row_scale(float sumsq, float amax, int D, float eps) {
     float rstd = 1.0f;
     if constexpr (OP == kNorm || OP == kNormAdd) rstd = 1.0f / sqrtf(sumsq / float(D) + eps);
     RowScale s;
-    s.scale = top == 0 ? 0.0f : amax * rstd / 127.0f;
+    s.scale = amax == 0.0f ? 0.0f : amax * rstd / 127.0f;
     s.zero = !(s.scale > 0.0f && s.scale < __uint_as_float(0x7f800000u));
     s.pre = amax < 7.8886091e-31f ? 18446744073709551616.0f : 1.0f;  // 2^-100, 2^64
     s.inv = 127.0f / (amax * s.pre);
     return s;
 }
 
+// A row so small that 127 / max would overflow is scaled up first.
+template <int N>
+__device__ __forceinline__ void prescale(const RowScale& s, float (&v)[N]) {
+    if (s.pre != 1.0f) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] *= s.pre;
+    }
+}
+
 // Sum and maximum over the G warps of a row (one warp: shuffles alone). Every
 // thread gets both; the order of the sum is fixed.
-__device__ __forceinline__ void reduce_row(float& sumsq, uint32_t& top, bool with_sum) {
+__device__ __forceinline__ void reduce_row(float& sumsq, float& amax, bool with_sum) {
     __shared__ float s_sum[32];
     __shared__ uint32_t s_top[32];
     if (with_sum) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sumsq += __shfl_xor_sync(0xffffffffu, sumsq, o);
     }
-    top = __reduce_max_sync(0xffffffffu, top);
+    // |v| as bits: unsigned order is that of the values, every NaN above infinity.
+    uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(amax) & 0x7fffffffu);
+    amax = __uint_as_float(top);
     const int G = blockDim.x >> 5;
     if (G == 1) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -177,6 +254,7 @@ __device__ __forceinline__ void reduce_row(float& sumsq, uint32_t& top, bool wit
     }
     __syncthreads();
     top = __reduce_max_sync(0xffffffffu, lane < G ? s_top[lane] : 0u);
+    amax = __uint_as_float(top);
     if (with_sum) {
         sumsq = lane < G ? s_sum[lane] : 0.0f;
 #pragma unroll
@@ -197,29 +275,32 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) ridge_row_i8(const RowParam
     const T* r = static_cast<const T*>(p.r) + (kR ? row * p.ldr : 0);
     const T* w = static_cast<const T*>(p.w);
     using C = Chunk<T, VEC>;
-    C cx[CH], cr[kR ? CH : 1];
     // Every load of the row is issued before the first value is used. The gain
-    // is not among them: all rows share it, so it comes from L1 or L2, and its
-    // registers would halve the rows in flight on an SM (112 against 64 registers
-    // a thread; 8192 x 8192 BF16 with a residual 136 us against 88 us).
+    // is among them where it is cheap. With four 16-byte chunks a thread it is not:
+    // its registers (112 against 64 a thread) would halve the rows in flight on an
+    // SM, and all rows share it, so it comes from L1 or L2 when it is needed
+    // (8192 x 8192 BF16 with a residual: 136 us with it early, 78 without).
+    constexpr bool kEarlyW = kW && (VEC == 1 ? CH <= 8 : CH <= 2);
+    C cx[CH], cr[kR ? CH : 1], cw[kEarlyW ? CH : 1];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int e = (c * int(blockDim.x) + int(threadIdx.x)) * VEC;
         if (e < p.D) {
             cx[c] = *reinterpret_cast<const C*>(x + e);
             if constexpr (kR) cr[c] = *reinterpret_cast<const C*>(r + e);
+            if constexpr (kEarlyW) cw[c] = *reinterpret_cast<const C*>(w + e);
         }
     }
     float v[CH][VEC];
     float sumsq = 0.0f;
-    uint32_t top = 0;
+    float top = 0.0f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int e = (c * int(blockDim.x) + int(threadIdx.x)) * VEC;
         if (e < p.D) {
-            C h, cw;
-            if constexpr (kW) cw = *reinterpret_cast<const C*>(w + e);
-            take_chunk<T, OP, VEC>(cx[c], cr[kR ? c : 0], cw, h, v[c], sumsq, top);
+            C h, gain = cw[kEarlyW ? c : 0];
+            if constexpr (kW && !kEarlyW) gain = *reinterpret_cast<const C*>(w + e);
+            take_chunk<T, OP, VEC>(cx[c], cr[kR ? c : 0], gain, h, v[c], sumsq, top);
             if constexpr (OP == kNormAdd)
                 *reinterpret_cast<C*>(static_cast<T*>(p.h) + row * p.ldh + e) = h;
         }
@@ -230,7 +311,8 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) ridge_row_i8(const RowParam
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int e = (c * int(blockDim.x) + int(threadIdx.x)) * VEC;
-        if (e < p.D) store_q<VEC>(q + e, v[c], s.pre, s.inv, s.zero);
+        prescale(s, v[c]);
+        if (e < p.D) store_q<VEC>(q + e, v[c], s.inv, s.zero);
     }
     if (threadIdx.x == 0) p.scale[row] = s.scale;
 }
@@ -250,7 +332,7 @@ __global__ void __launch_bounds__(1024) ridge_row_i8_long(const RowParams p) {
     using C = Chunk<T, VEC>;
     const int64_t step = int64_t(blockDim.x) * VEC;
     float sumsq = 0.0f;
-    uint32_t top = 0;
+    float top = 0.0f;
     C cx, cr, cw, h;
     float v[VEC];
     auto load = [&](int64_t e) {
@@ -266,13 +348,14 @@ __global__ void __launch_bounds__(1024) ridge_row_i8_long(const RowParams p) {
     const RowScale s = row_scale<OP>(sumsq, top, p.D, p.eps);
     int8_t* q = p.q + row * p.ldq;
     float unused_sum = 0.0f;
-    uint32_t unused_top = 0;
+    float unused_top = 0.0f;
     for (int64_t e = int64_t(threadIdx.x) * VEC; e < p.D; e += step) {
         load(e);
         take_chunk<T, OP, VEC>(cx, cr, cw, h, v, unused_sum, unused_top);
         if constexpr (OP == kNormAdd)
             *reinterpret_cast<C*>(static_cast<T*>(p.h) + row * p.ldh + e) = h;
-        store_q<VEC>(q + e, v, s.pre, s.inv, s.zero);
+        prescale(s, v);
+        store_q<VEC>(q + e, v, s.inv, s.zero);
     }
     if (threadIdx.x == 0) p.scale[row] = s.scale;
 }
@@ -307,6 +390,8 @@ cudaError_t run_rows(const RowParams& p, int num_sms, cudaStream_t stream) {
     } else {
         if (chunks <= 128) return launch_rows<T, OP, VEC, 4, 1024>(p, 32, 4, stream);
         if (chunks <= 4096) return launch_rows<T, OP, VEC, 4, 1024>(p, threads_for(4), 1, stream);
+        if (p.M <= num_sms && chunks <= 8192)
+            return launch_rows<T, OP, VEC, 8, 1024>(p, threads_for(8), 1, stream);
         if (chunks <= 16384) return launch_rows<T, OP, VEC, 16, 1024>(p, threads_for(16), 1, stream);
     }
     ridge_row_i8_long<T, OP, VEC><<<unsigned(p.M), 1024, 0, stream>>>(p);

@@ -78,9 +78,11 @@ __global__ void __launch_bounds__(256)
             constexpr int V = kVecOf<T>;
 #pragma unroll
             for (int g = 0; g < 16 / V; ++g) {
-                Chunk<T, V> o;
+                float f[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) o.e[i] = from_f32<T>(float(in.e[g * V + i]) * s);
+                for (int i = 0; i < V; ++i) f[i] = float(in.raw[g * V + i]) * s;
+                Chunk<T, V> o;
+                o.set(f);
                 *reinterpret_cast<Chunk<T, V>*>(dst + e + g * V) = o;
             }
         } else {

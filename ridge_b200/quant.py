@@ -25,14 +25,21 @@ import math
 
 from ._native import RIDGE_BF16, RIDGE_F16, RIDGE_F32, check, lib
 
-_TYPES = None
+torch = None    # imported by the first call: the package itself does not need it
+_TYPES = {}
+
+
+def _need_torch():
+    global torch
+    import torch as module
+    _TYPES.update({module.float16: RIDGE_F16, module.bfloat16: RIDGE_BF16,
+                   module.float32: RIDGE_F32})
+    torch = module
 
 
 def _type_code(dtype, what):
-    global _TYPES
-    if _TYPES is None:
-        import torch
-        _TYPES = {torch.float16: RIDGE_F16, torch.bfloat16: RIDGE_BF16, torch.float32: RIDGE_F32}
+    if torch is None:
+        _need_torch()
     code = _TYPES.get(dtype)
     if code is None:
         raise TypeError("%s is float16, bfloat16 or float32, not %s" % (what, dtype))
@@ -76,7 +83,6 @@ def _vector(t, what, device, dtype, n):
 def _run(device, stream, call):
     """call(handle) with the tensors' device current; on a stream other than torch's
     current one, inside that stream's context, so that outputs come from its pool."""
-    import torch
     index = device.index
     if stream is None and torch._C._cuda_getDevice() == index:
         return call(torch._C._cuda_getCurrentRawStream(index))
@@ -93,13 +99,11 @@ def _run(device, stream, call):
 
 
 def _new(shape, strides, dtype, device):
-    import torch
     return torch.empty_strided(shape, strides, dtype=dtype, device=device)
 
 
 def _given(M, D, device, out, scale):
     """Checks the arrays that a caller passed for (q, scale)."""
-    import torch
     if out is not None:
         _like(out, "out", device, torch.int8, (M, D))
         _rows(out, "out")
@@ -109,7 +113,6 @@ def _given(M, D, device, out, scale):
 
 def _outputs(M, D, device, out, scale):
     """(q, q's pitch, scale): the given arrays or new ones."""
-    import torch
     if out is None:
         pitch = (D + 15) // 16 * 16
         out = _new((M, D), (pitch, 1), torch.int8, device)
@@ -206,7 +209,8 @@ def silu_mul_i8(gate, up, out=None, scale=None, stream=None):
 def dequantize_i8(q, scale, out=None, dtype=None, stream=None):
     """The values scale[i] * q[i, j], rounded once to dtype (float16 by default,
     or that of `out`)."""
-    import torch
+    if torch is None:
+        _need_torch()
     if q.dtype != torch.int8:
         raise TypeError("q is int8, got %s" % q.dtype)
     M, D, ldq = _rows(q, "q")
@@ -237,7 +241,8 @@ def gemm_i8(a, a_scale, b, b_scale, bias=None, out=None, dtype=None, stream=None
     calls return them; out (M, N) float16 (default), bfloat16 or float32, bias (N,)
     of that type. The integer sum is exact (K < 131072). a and b start on 16 bytes
     and their row pitches are multiples of 16 (RidgeError otherwise)."""
-    import torch
+    if torch is None:
+        _need_torch()
     if a.dtype != torch.int8 or b.dtype != torch.int8:
         raise TypeError("ridge_b200.gemm_i8 takes int8 operands")
     M, K, lda = _rows(a, "a")
