@@ -380,22 +380,38 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
             }
         };
 
-        I8Item w;
-        for (int it = unit; i8_item(p, it, num_m, num_n, w); it += num_units) {
+        // An item's scales and biases go through registers to shared memory, fetched
+        // while the item before it is drained: read from global memory in the drain
+        // itself they made a 256 x 256 tile's epilogue 6.4 us long.
+        constexpr int kFetch = kI8TileCols / 32;
+        float next_sa = 0.0f, next_sb[kFetch], next_bias[kFetch];
+        I8Item w, next;
+        auto fetch = [&](const I8Item& t) {
+            const int row = t.tm * 256 + int(rank) * 128 + quad * 32 + lane;
+            next_sa = row < p.M ? p.sa[row] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < kFetch; ++i) {
+                const int col = t.col + (group + 2 * (i / 2)) * 64 + (i % 2) * 32 + lane;
+                next_sb[i] = col < p.N ? p.sb[col] : 0.0f;
+                next_bias[i] = bias && col < p.N ? OutType<T>::up(bias[col]) : 0.0f;
+            }
+        };
+        bool more = i8_item(p, unit, num_m, num_n, next);
+        if (more) fetch(next);
+        for (int it = unit; more; it += num_units) {
+            w = next;
             const int units = w.width / 64;
             const int row0 = w.tm * 256 + int(rank) * 128 + quad * 32;
-            const float row_scale = row0 + lane < p.M ? p.sa[row0 + lane] : 0.0f;
-            // Fetched while the tile's MMAs still run: read from global memory in
-            // the drain itself they made a 256 x 256 tile's epilogue 6.4 us long.
+            const float row_scale = next_sa;
             __syncwarp();
 #pragma unroll
-            for (int i = 0; i < kI8TileCols / 32; ++i) {
-                const int col = w.col + (group + 2 * (i / 2)) * 64 + (i % 2) * 32 + lane;
-                const bool in = col < p.N;
-                cols[i * 32 + lane] = in ? p.sb[col] : 0.0f;
-                if (bias) cols[kI8TileCols + i * 32 + lane] = in ? OutType<T>::up(bias[col]) : 0.0f;
+            for (int i = 0; i < kFetch; ++i) {
+                cols[i * 32 + lane] = next_sb[i];
+                if (bias) cols[kI8TileCols + i * 32 + lane] = next_bias[i];
             }
             __syncwarp();
+            more = i8_item(p, it + num_units, num_m, num_n, next);
+            if (more) fetch(next);
             int ok = 1;
             if (lane == 0)
                 ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.err, kErrTimeoutEpilogue);
@@ -689,11 +705,11 @@ __global__ void __launch_bounds__(kI8StreamThreads)
         const float4 channel = *reinterpret_cast<const float4*>(channel_scale + lane * 4);
         const float4 b = *reinterpret_cast<const float4*>(channel_bias + lane * 4);
         const int live = min(bn, p.M - t0);  // tokens of this tile
+        // The other ranks' sums, and this CTA's own without the way over the cluster.
         uint32_t peer[SPLIT];
+        peer[0] = base + uint32_t(lane * 16);
 #pragma unroll
-        for (int s = 0; s < SPLIT; ++s)
-            peer[s] = SPLIT > 1 ? map_to_cta(base + uint32_t(lane * 16), s)
-                                : base + uint32_t(lane * 16);
+        for (int s = 1; s < SPLIT; ++s) peer[s] = map_to_cta(peer[0], uint32_t((rank + s) % SPLIT));
         constexpr int kStep = (kI8StreamThreads / 32) * SPLIT;  // tokens between two of a warp's
         constexpr int kFlight = SPLIT >= 8 ? 2 : SPLIT >= 4 ? 4 : 8;
         for (int t = rank + warp * SPLIT; t < live; t += kFlight * kStep) {
@@ -703,9 +719,10 @@ __global__ void __launch_bounds__(kI8StreamThreads)
                 const int ti = t + i * kStep;
                 sum[i] = make_int4(0, 0, 0, 0);
                 if (ti < live) {
+                    sum[i] = ld_sums<false>(peer[0] + uint32_t(ti) * 512u);
 #pragma unroll
-                    for (int s = 0; s < SPLIT; ++s) {
-                        const int4 v = ld_sums<(SPLIT > 1)>(peer[s] + uint32_t(ti) * 512u);
+                    for (int s = 1; s < SPLIT; ++s) {
+                        const int4 v = ld_sums<true>(peer[s] + uint32_t(ti) * 512u);
                         sum[i].x += v.x;
                         sum[i].y += v.y;
                         sum[i].z += v.z;
