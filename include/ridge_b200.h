@@ -305,11 +305,12 @@ int ridge_dequantize_i8(const int8_t* q, const float* scale, int32_t type, void*
  *   bias     N elements of `type`, or NULL
  *   C        M x N of `type`, pitch ldc elements (>= N)
  * The sum is a 32-bit integer, exact for every K < 2^17 (longer K is refused with
- * RIDGE_EINVAL, as are M or N above 2^30); it is rounded to FP32, scaled there, and rounded once more to
- * `type`. A and B start on 16 bytes and lda, ldb are multiples of 16 (TMA); a
- * pitch is ignored where there is one row. C needs only its elements' alignment, and pitch and bytes past column N are
- * not touched. K may be 0 (C is then the bias, or 0). C overlaps no input. The
- * tile is chosen from M, N, K and the device; results do not depend on it.
+ * RIDGE_EINVAL, as are M or N above 2^30); it is rounded to FP32, scaled there,
+ * and rounded once more to `type`. A and B start on 16 bytes and lda, ldb are
+ * multiples of 16 (TMA); a pitch is ignored where there is one row. C needs only
+ * its elements' alignment; what lies between a row's column N and the next row
+ * is not touched. K may be 0 (C is then the bias, or 0). C overlaps no input.
+ * The tile is chosen from M, N, K and the device; results do not depend on it.
  * Asynchronous on `stream`; needs no workspace and can be captured into a graph.
  * Kernels use the bounded waits and the error word of the other launches
  * (ridge_device_error).

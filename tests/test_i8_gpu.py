@@ -11,8 +11,8 @@ quantising: scale is one division away from max|y|, q is the whole number neares
 norm: rstd = 1 / sqrt(sumsq / D + eps); a thread adds up to T squares one after the other,
   then at most 10 + 5 levels of pairs, all positive: relative error (T + 15 + 3) u, halved by
   the square root, plus 4 u for its own steps; scale adds 2 e + 2 u.
-activation: __expf is within 2 + 1.173 |x| units of 2^-23, __fdividef within 2 units, then an
-  addition and a product.
+activation: e^-x within 2 + 1.173 |x| units of 2^-23 (an exponent rounded in FP32, then the
+  hardware's ex2), a reciprocal within 2 units, then an addition and two products.
 gemm: the integer is exact; FP32 rounds it, its product with sb and the final fused
   multiply-add: 2 u of the product and u of the result, plus one rounding to the type.
 """
@@ -248,6 +248,17 @@ def test_gemm_shapes(shape, dtype):
     assert torch.equal(out.view(torch.uint8), again.view(torch.uint8))
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape", [(3840, 1280, 256), (3840, 1270, 2100), (2304, 2400, 700),
+                                   (19000, 300, 96), (5000, 5000, 128)],
+                         ids=lambda s: "%dx%dx%d" % s)
+def test_gemm_more_tiles_than_pairs(shape, dtype):
+    """Several rounds of tiles, the last of them few (75 or 90 tiles of 256 x 256) or many."""
+    a, sa, b, sb = _operands(*shape, seed=8)
+    bias = _rand((shape[1],), dtype, 9)
+    _check_gemm(rb.gemm_i8(a, sa, b, sb, bias=bias, dtype=dtype), a, sa, b, sb, bias)
+
+
 @pytest.mark.parametrize("M", [3, 200, 600])
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_gemm_output_pitch_and_alignment(M, dtype):
@@ -362,6 +373,36 @@ def test_two_products_at_once():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def test_beside_the_fp16_family():
+    """Products of both families on two streams: they share SMs and Tensor Memory."""
+    c = _operands(20, 4096, 2048, 7)
+    want = rb.gemm_i8(*c)
+    a, b = _rand((700, 1024), torch.float16, 1), _rand((900, 1024), torch.float16, 2)
+    pair = rb.TileConfig(256, 256, 32, 2, 4, 8, 2)
+    want16 = rb.gemm(a, b, config=pair)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got, got16 = [], []
+    for _ in range(8):
+        got.append(rb.gemm_i8(*c, stream=streams[0]))
+        with torch.cuda.stream(streams[1]):
+            got16.append(rb.gemm(a, b, config=pair))
+    torch.cuda.synchronize()
+    assert rb.device_error() == 0
+    assert all(torch.equal(g, want) for g in got)
+    assert all(torch.equal(g, want16) for g in got16)
+
+
+def test_the_same_tensor_twice():
+    """One tensor as both inputs of the addition, and as both operands of a product."""
+    x = _rand((12, 640), torch.bfloat16, 3)
+    w = torch.ones(640, dtype=torch.bfloat16, device="cuda")
+    q, s, h = rb.rms_norm_i8(x, w, residual=x.clone())
+    q2, s2, _ = rb.rms_norm_i8(x, w, residual=x, residual_out=x)
+    assert torch.equal(q, q2) and torch.equal(s, s2) and torch.equal(h, x)
+    _check_gemm(rb.gemm_i8(q, s, q, s, dtype=torch.float32), q, s, q, s, None)
 
 
 @pytest.mark.parametrize("M", [1, 9, 300])
