@@ -123,15 +123,16 @@ double stream_time(const Plan& p, int64_t num_kb, int num_sms) {
     return 4.2 + waves * out + steps * std::max((p.sub == 2 ? 0.23 : 0.26) * waves, feed * per_sm);
 }
 
-// A pair takes 0.35 to 0.38 us for a K block, little less for narrow tiles, and
-// 2.4 us to drain 256 columns, which bounds a tile of few K blocks.
+// A pair takes 0.35 to 0.38 us for a K block, little less for narrow tiles (5%
+// more for strips, whose ring is no deeper than that of the tiles they are cut
+// from), and 2.4 us to drain 256 columns, which bounds a tile of few K blocks.
 double tile_time(const Plan& p, int64_t num_kb, int pairs) {
     auto round = [&](int width) {
         const double block = width == 256 ? 0.38 : width == 192 ? 0.36 : 0.35;
         return std::max(block * num_kb, 2.4 * width / 256);
     };
     const int64_t rounds = p.cut > 1 ? p.whole / pairs : ceil_div(p.items, pairs);
-    return 7.4 + rounds * round(p.bn) + (p.cut > 1 ? round(p.bn / p.cut) : 0.0);
+    return 7.4 + rounds * round(p.bn) + (p.cut > 1 ? 1.05 * round(p.bn / p.cut) : 0.0);
 }
 
 // The kernel and tile with the least estimated time. Sums are exact integers, so
