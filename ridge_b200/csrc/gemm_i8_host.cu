@@ -79,8 +79,8 @@ int stream_residents(int bn, int blocks) {
 
 // Up to `bn` tokens to a tile, evened out over the tiles, and the ring: all of
 // the shared memory when every CTA can have an SM to itself, else half of it
-// where that leaves three stages.
-Plan stream_plan(int64_t M, int64_t N, int bn, int split, int num_sms) {
+// where that leaves three K blocks.
+Plan stream_plan(int64_t M, int64_t N, int64_t K, int bn, int split, int num_sms) {
     Plan p{};
     p.stream = true;
     p.split = split;
@@ -98,19 +98,24 @@ Plan stream_plan(int64_t M, int64_t N, int bn, int split, int num_sms) {
         const int half = stages_for(stage, fixed, kSmemPerSm / 2 - kSmemReservedPerCta);
         if (half * p.sub >= 3) p.stages = half;
     }
+    // No more than K fills, so that short products leave room for more CTAs, but
+    // enough to hold the sums of the tile (bn tokens x 128 channels) at the end.
+    const int64_t steps = ceil_div(ceil_div(ceil_div(K, kI8BK), split), p.sub);
+    const int64_t sums = ceil_div(int64_t(p.bn) * 512, stage);
+    p.stages = int(std::min<int64_t>(p.stages, std::max(steps, sums)));
     return p;
 }
 
-// Estimated times in microseconds, good for ranking plans: fitted to 2,656 timed
-// launches of 107 shapes (1 to 8192 tokens, K of 256 to 16384, every tile, split
-// and ring below). The plan they pick is on average 1.5% slower than the best of a
-// shape, 12% at worst.
+// Estimated times in microseconds, good for ranking plans: fitted to some 2,700
+// timed launches of 107 shapes (1 to 8192 tokens, K of 256 to 16384, every tile,
+// split and ring below) and 20 more with K from 64. The plans they pick are on
+// average within 1% of the best of a shape.
 //
 // A streaming CTA takes 0.26 us for a K block of its own (0.23 with two to a
-// stage) and an SM takes in
-// 97 bytes/ns for all of its CTAs; sums leave at 20 ns a token, over a cluster
-// with 1 us + 70 ns a rank for the exchange. Clusters of 4 and 8 do not find
-// room on every SM.
+// stage) and an SM takes in 97 bytes/ns for all of its CTAs; sums leave at 20 ns a
+// token, over a cluster with 1 us + 70 ns a rank for the exchange; each wave of
+// CTAs after the first takes 0.8 us to start. Clusters of 4 and 8 do not find room
+// on every SM.
 double stream_time(const Plan& p, int64_t num_kb, int num_sms) {
     const double room = p.split == 8 ? 0.757 : p.split == 4 ? 0.892 : 1.0;
     const int64_t at_once = std::max<int64_t>(
@@ -120,29 +125,37 @@ double stream_time(const Plan& p, int64_t num_kb, int num_sms) {
     const double steps = double(ceil_div(num_kb, p.split));
     const double out = (p.split > 1 ? 1.0 + 0.07 * p.split : 0.25) + 0.02 * p.bn;
     const double feed = i8_stream_block_bytes(p.bn) / 97e3;
-    return 4.2 + waves * out + steps * std::max((p.sub == 2 ? 0.23 : 0.26) * waves, feed * per_sm);
+    const double step = p.sub == 2 ? 0.23 : 0.26;
+    return 3.4 + waves * (0.8 + out) + steps * std::max(step * waves, feed * per_sm);
 }
 
 // A pair takes 0.35 to 0.38 us for a K block, little less for narrow tiles (5%
 // more for strips, whose ring is no deeper than that of the tiles they are cut
-// from), and 2.4 us to drain 256 columns, which bounds a tile of few K blocks.
-double tile_time(const Plan& p, int64_t num_kb, int pairs) {
-    auto round = [&](int width) {
+// from), and 1.5 us + 5.5 ns a column to drain a tile into 16-bit C, 1.45 times
+// that into 32-bit C. The drain of a tile overlaps the next one's K blocks.
+double tile_time(const Plan& p, int64_t num_kb, int elem_size, int pairs) {
+    double shorter = 0;
+    auto round = [&](int width, double extra) {
         const double block = width == 256 ? 0.38 : width == 192 ? 0.36 : 0.35;
-        return std::max(block * num_kb, 2.4 * width / 256);
+        const double blocks = block * num_kb * extra;
+        const double drain = (1.5 + 0.0055 * width) * (elem_size == 4 ? 1.45 : 1.0);
+        shorter = std::min(blocks, drain);
+        return std::max(blocks, drain);
     };
     const int64_t rounds = p.cut > 1 ? p.whole / pairs : ceil_div(p.items, pairs);
-    return 7.4 + rounds * round(p.bn) + (p.cut > 1 ? 1.05 * round(p.bn / p.cut) : 0.0);
+    double t = 4.6 + rounds * round(p.bn, 1.0);
+    if (p.cut > 1) t += round(p.bn / p.cut, 1.05);
+    return t + shorter;
 }
 
 // The kernel and tile with the least estimated time. Sums are exact integers, so
 // results do not depend on the choice.
-Plan make_plan(int64_t M, int64_t N, int64_t K, int num_sms, int pairs) {
+Plan make_plan(int64_t M, int64_t N, int64_t K, int elem_size, int num_sms, int pairs) {
 #ifdef RIDGE_I8_PROBE
     if (const char* v = std::getenv("RIDGE_I8_PLAN")) {
         int s = 0, bn = 0, stages = 0, split = 0, sub = 1;
         std::sscanf(v, "%d,%d,%d,%d,%d", &s, &bn, &stages, &split, &sub);
-        Plan p = s ? stream_plan(M, N, bn, split, num_sms) : tile_plan(M, N, bn, pairs);
+        Plan p = s ? stream_plan(M, N, K, bn, split, num_sms) : tile_plan(M, N, bn, pairs);
         p.stages = stages;
         p.sub = sub;
         return p;
@@ -159,12 +172,12 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int num_sms, int pairs) {
     };
     for (int bn : {256, 192, 128, 64}) {
         const Plan p = tile_plan(M, N, bn, pairs);
-        offer(p, tile_time(p, num_kb, pairs));
+        offer(p, tile_time(p, num_kb, elem_size, pairs));
     }
     for (int bn : {64, 128, 256}) {
         if (ceil_div(M, bn) > 65535) continue;  // the grid's second dimension
         for (int split = 1; split <= 8 && split <= num_kb; split *= 2) {
-            const Plan p = stream_plan(M, N, bn, split, num_sms);
+            const Plan p = stream_plan(M, N, K, bn, split, num_sms);
             offer(p, stream_time(p, num_kb, num_sms));
         }
         if (M <= bn) break;  // one token tile already
@@ -281,7 +294,7 @@ int run_product(const int8_t* A, const int8_t* B, int32_t type, int64_t lda, int
     int pairs = 0;
     int st = resident_pairs<T>(dev, &pairs);
     if (st != RIDGE_OK) return st;
-    const Plan plan = make_plan(p.M, p.N, p.K, dev.num_sms, pairs);
+    const Plan plan = make_plan(p.M, p.N, p.K, int(sizeof(T)), dev.num_sms, pairs);
     p.bn = plan.bn;
     p.stages = plan.stages;
     p.sub = plan.sub;
@@ -300,7 +313,10 @@ int run_product(const int8_t* A, const int8_t* B, int32_t type, int64_t lda, int
         }
     }
     if (plan.items > int64_t(1) << 30) return RIDGE_EINVAL;
-    p.groupM = 8;
+    // Row tiles taken together: 16 share more of B in L2 while K is long (8192^3 328
+    // us against 340 with 8), 8 write C in a better order while it is short
+    // (8192 x 8192 x 512 50 us against 54.6).
+    p.groupM = p.K >= 4096 ? 16 : 8;
     p.whole = plan.whole;
     p.cut = plan.cut;
     CUtensorMap strip = b, c;

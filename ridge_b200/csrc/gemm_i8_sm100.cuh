@@ -111,13 +111,6 @@ __device__ __forceinline__ void i8_let_loads_land() {
     }
 }
 
-// Where a tile or split starts in its K range: tiles that share a panel would
-// otherwise read the same lines of it at the same moment, and a few lines do not
-// spread over the L2 slices. The integer sum does not depend on the order.
-__device__ __forceinline__ int i8_first_block(int seed, int num_kb) {
-    return num_kb < 16 ? seed % num_kb : seed & 15;
-}
-
 // One unit of work of the tile kernel: rows from 256 * tm, columns [col, col + width).
 struct I8Item {
     int tm, tn, col, width;
@@ -226,8 +219,7 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
             const int b_row = w.col + int(rank) * rows_b;
             const void* map_b = w.width == bn ? &tmap_b : &tmap_strip;
             const uint32_t bytes = uint32_t(i8_tile_stage_bytes(w.width));
-            int kb = i8_first_block(3 * w.tm + 5 * w.tn, num_kb);
-            for (int i = 0; i < num_kb; ++i) {
+            for (int kb = 0; kb < num_kb; ++kb) {
                 if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.err,
                                kErrTimeoutProducer)) {
                     ok = false;
@@ -241,7 +233,6 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
                 } else {
                     tma_load_2d_pair(sa + 128 * kI8BK, map_b, fb, kb * kI8BK, b_row);
                 }
-                if (++kb == num_kb) kb = 0;
                 if (++stage == stages) {
                     stage = 0;
                     phase ^= 1u;
@@ -550,7 +541,11 @@ __global__ void __launch_bounds__(kI8StreamThreads)
     const int blocks = kb1 - kb0;
     const int steps = (blocks + sub - 1) / sub;
     // K block of this CTA's i-th place, and the loads of a step: B arms the stage.
-    const int turn = i8_first_block(3 * int(blockIdx.x / SPLIT) + 5 * int(blockIdx.y), blocks);
+    // CTAs start at different places of their K range (the sum does not depend on
+    // the order): 1 x 8192 x 8192 14.3 us, against 14.9 with all in step. Tiles of
+    // the other kernel share panels and are 2 to 5% faster in step.
+    const int spread = 3 * int(blockIdx.x / SPLIT) + 5 * int(blockIdx.y);
+    const int turn = blocks < 16 ? spread % blocks : spread & 15;
     auto block_of = [&](int i) {
         const int kb = kb0 + turn + i;
         return kb < kb1 ? kb : kb - blocks;
