@@ -90,7 +90,7 @@ struct OutType<float> {
 
 // ------------------------------------------------------------------ tiles by 2-CTA pairs
 
-constexpr int kI8TileThreads = 11 * 32;  // A producer, MMA, 8 epilogue warps, B producer
+constexpr int kI8TileThreads = 10 * 32;  // producer, MMA, 8 epilogue warps
 constexpr int kI8TileStageOut = 4096;  // 32 rows x 128 bytes of C per epilogue warp
 constexpr int kI8TileCols = 2 * 64;    // columns of a tile that one epilogue warp drains
 constexpr int kI8TileEpiBytes = 8 * (kI8TileStageOut + kI8TileCols * 8);
@@ -102,13 +102,13 @@ constexpr int i8_tile_smem(int bn, int stages) {
     return kI8AlignSlack + stages * i8_tile_stage_bytes(bn) + kI8TileEpiBytes + kI8BarrierBytes;
 }
 
-// Abort path of a producer: its loads in flight (which take microseconds) land
-// before the CTA can exit. A timed wait, since the stage they complete may never
-// be armed once the other producer has given up too.
-__device__ __forceinline__ void i8_let_loads_land() {
-    const uint64_t t0 = global_timer_ns();
-    while (global_timer_ns() - t0 < 2000000ull) {
-    }
+// Abort path of a producer that has filled `issued` stages in turn: the loads in
+// flight, at most one filling of each ring slot, land before the CTA can exit.
+__device__ __forceinline__ void i8_drain_loads(uint32_t full_bar0, int stages, long long issued,
+                                               int* err) {
+    for (long long i = issued > stages ? issued - stages : 0; i < issued; ++i)
+        mbar_wait(full_bar0 + 8u * uint32_t(i % stages), uint32_t((i / stages) & 1), nullptr, err,
+                  kErrTimeoutDrain);
 }
 
 // One unit of work of the tile kernel: rows from 256 * tm, columns [col, col + width).
@@ -202,15 +202,12 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
     const int unit = blockIdx.x / 2;
     const int num_units = gridDim.x / 2;
 
-    if ((warp == 0 || warp == 10) && lane == 0) {
-        // ------------------------------------------------------ TMA producers
-        // Warp 0 loads A and arms the stage, warp 10 loads B. A load may complete
-        // before its phase is armed; the phase cannot finish before the arming
-        // thread arrives.
-        const bool loads_a = warp == 0;
+    if (warp == 0 && lane == 0) {
+        // ------------------------------------------------------ TMA producer
         const uint32_t leader_full0 = map_to_cta(full_bar(0), 0);
         int stage = 0;
         uint32_t phase = 0;
+        long long issued = 0;
         bool ok = true;
         I8Item w;
         for (int it = unit; ok && i8_item(p, it, num_m, num_n, w); it += num_units) {
@@ -227,19 +224,19 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
                 }
                 const uint32_t sa = base + stage * stage_bytes;
                 const uint32_t fb = leader_full0 + 8u * uint32_t(stage);
-                if (loads_a) {
-                    if (leader) mbar_arrive_expect_tx(full_bar(stage), 2 * bytes);
-                    tma_load_2d_pair(sa, &tmap_a, fb, kb * kI8BK, a_row);
-                } else {
-                    tma_load_2d_pair(sa + 128 * kI8BK, map_b, fb, kb * kI8BK, b_row);
-                }
+                if (leader) mbar_arrive_expect_tx(full_bar(stage), 2 * bytes);
+                tma_load_2d_pair(sa, &tmap_a, fb, kb * kI8BK, a_row);
+                tma_load_2d_pair(sa + 128 * kI8BK, map_b, fb, kb * kI8BK, b_row);
+                ++issued;
                 if (++stage == stages) {
                     stage = 0;
                     phase ^= 1u;
                 }
             }
         }
-        if (!ok) i8_let_loads_land();
+        // The leader's barriers count the follower's bytes too, and neither CTA
+        // leaves before the last cluster barrier.
+        if (!ok && leader) i8_drain_loads(full_bar(0), stages, issued, p.err);
     } else if (warp == 1 && leader) {
         // ------------------------------------------------------ MMA issuer
         // The whole warp walks the ring and one elected lane issues: with every
@@ -289,7 +286,7 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
             umma_commit_pair(drain_bar, 0x1);
             mbar_wait(drain_bar, 0, nullptr, p.err, kErrTimeoutDrain);
         }
-    } else if (warp >= 2 && warp < 10) {
+    } else if (warp >= 2) {
         // ------------------------------------------------------ epilogue
         // A warp drains 32 rows x 64 columns at a time (two column groups of four
         // warps take alternate 64s): TMEM -> registers -> scaled -> 4 KB of
@@ -458,7 +455,7 @@ __global__ void __launch_bounds__(kI8TileThreads, 1)
 
 // ------------------------------------------------------------------ B streamed past few rows of A
 
-constexpr int kI8StreamThreads = 7 * 32;  // B producer, MMA, 4 epilogue warps, A producer
+constexpr int kI8StreamThreads = 6 * 32;  // producer, MMA, 4 epilogue warps
 
 constexpr int kI8StreamScales = (256 + 128 + 128) * 4;  // token and channel scales, biases
 
@@ -540,33 +537,27 @@ __global__ void __launch_bounds__(kI8StreamThreads)
     const int kb1 = int((long long)num_kb * (rank + 1) / SPLIT);
     const int blocks = kb1 - kb0;
     const int steps = (blocks + sub - 1) / sub;
-    // K block of this CTA's i-th place, and the loads of a step: B arms the stage.
-    // CTAs start at different places of their K range (the sum does not depend on
-    // the order): 1 x 8192 x 8192 14.3 us, against 14.9 with all in step. Tiles of
-    // the other kernel share panels and are 2 to 5% faster in step.
+    // K block of this CTA's i-th place, and the loads of a step. CTAs start at
+    // different places of their K range (the sum does not depend on the order):
+    // 1 x 8192 x 8192 14.3 us, against 14.9 with all in step. Tiles of the other
+    // kernel share panels and are 2 to 5% faster in step.
     const int spread = 3 * int(blockIdx.x / SPLIT) + 5 * int(blockIdx.y);
     const int turn = blocks < 16 ? spread % blocks : spread & 15;
-    auto block_of = [&](int i) {
-        const int kb = kb0 + turn + i;
-        return kb < kb1 ? kb : kb - blocks;
-    };
-    auto load_b = [&](int stage, int step) {
+    auto load = [&](int stage, int step) {
         const int n = min(sub, blocks - step * sub);
         mbar_arrive_expect_tx(full_bar(stage), uint32_t(n) * block_bytes);
-        for (int j = 0; j < n; ++j)
-            tma_load_2d(base + stage * stage_bytes + j * block_bytes, &tmap_b, full_bar(stage),
-                        block_of(step * sub + j) * kI8BK, f0);
-    };
-    auto load_a = [&](int stage, int step) {
-        const int n = min(sub, blocks - step * sub);
-        for (int j = 0; j < n; ++j)
-            tma_load_2d(base + stage * stage_bytes + j * block_bytes + 128 * kI8BK, &tmap_a,
-                        full_bar(stage), block_of(step * sub + j) * kI8BK, t0);
+        for (int j = 0; j < n; ++j) {
+            const int place = kb0 + turn + step * sub + j;
+            const int x = (place < kb1 ? place : place - blocks) * kI8BK;
+            const uint32_t at = base + stage * stage_bytes + j * block_bytes;
+            tma_load_2d(at, &tmap_b, full_bar(stage), x, f0);
+            tma_load_2d(at + 128 * kI8BK, &tmap_a, full_bar(stage), x, t0);
+        }
     };
 
-    if (threadIdx.x == 32 * 6) tma_prefetch_desc(&tmap_a);
     if (threadIdx.x == 0) {
         tma_prefetch_desc(&tmap_b);
+        tma_prefetch_desc(&tmap_a);
         for (int s = 0; s < stages; ++s) {
             mbar_init(full_bar(s), 1);
             mbar_init(empty_bar(s), 1);
@@ -575,9 +566,8 @@ __global__ void __launch_bounds__(kI8StreamThreads)
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
         fence_barrier_init();
-        // The first stages of B, the bulk of the bytes, do not wait for the rest
-        // of the set-up.
-        for (int s = 0; s < min(stages, steps); ++s) load_b(s, s);
+        // The first loads do not wait for the rest of the set-up.
+        for (int s = 0; s < min(stages, steps); ++s) load(s, s);
     }
     if (warp == 1) {
         tmem_alloc<1>(smem_u32(tmem_slot), tmem_cols);
@@ -593,30 +583,21 @@ __global__ void __launch_bounds__(kI8StreamThreads)
     const T* bias = static_cast<const T*>(p.bias);
     T* C = static_cast<T*>(p.C);
 
-    if ((warp == 0 || warp == 6) && lane == 0) {
-        // Warp 0 loads B and arms the stage, warp 6 loads A. A load may complete
-        // before its phase is armed; the phase cannot finish before the arming
-        // thread arrives. B's first stages are under way already.
-        const bool loads_b = warp == 0;
-        const int first = loads_b ? min(stages, steps) : 0;
+    if (warp == 0 && lane == 0) {
+        const int first = min(stages, steps);  // under way already
         int stage = first == stages ? 0 : first;
         uint32_t phase = first == stages ? 1u : 0u;
-        bool live = true;
-        for (int i = first; i < steps; ++i) {
-            if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.err, kErrTimeoutProducer)) {
-                live = false;
+        int i = first;
+        for (; i < steps; ++i) {
+            if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.err, kErrTimeoutProducer))
                 break;
-            }
-            if (loads_b)
-                load_b(stage, i);
-            else
-                load_a(stage, i);
+            load(stage, i);
             if (++stage == stages) {
                 stage = 0;
                 phase ^= 1u;
             }
         }
-        if (!live) i8_let_loads_land();
+        if (i < steps) i8_drain_loads(full_bar(0), stages, i, p.err);
     } else if (warp == 1) {
         const uint32_t idesc = make_idesc_i8_s32(128, bn);
         int stage = 0;
@@ -654,7 +635,7 @@ __global__ void __launch_bounds__(kI8StreamThreads)
                 mbar_wait(drain_bar, 0, nullptr, p.err, kErrTimeoutDrain);
             }
         }
-    } else if (warp >= 2 && warp < 6) {
+    } else if (warp >= 2) {
         for (int i = int(threadIdx.x) - 64; i < bn; i += 128)
             token_scale[i] = t0 + i < p.M ? p.sa[t0 + i] : 0.0f;
         {
