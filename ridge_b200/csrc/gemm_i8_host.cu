@@ -281,6 +281,32 @@ int launch_stream(const Plan& plan, const CUtensorMap& a, const CUtensorMap& b,
     return int(cudaLaunchKernelEx(&cfg, ridge_gemm_i8_stream<T, SPLIT>, a, b, p));
 }
 
+// Products that go to ridge_gemm_i8_vec: one token while B is at most 64 MB, two
+// tokens 16 MB, four 8 MB, the latter with at most 4096 channels. At the edges,
+// against the streaming kernel: 1 x 8192 x 8192 13.6 us to 13.8, 1 x 14336 x 4096
+// 13.2 to 12.3; 2 x 4096 x 4096 5.9 to 6.9, 2 x 8192 x 8192 14.6 to 13.9, 2 x 11008 x
+// 512 4.3 to 3.8; 4 x 1024 x 4096 3.5 to 4.9, 4 x 4096 x 4096 7.8 to 7.0.
+bool vec_serves(int64_t M, int64_t N, int64_t K) {
+    const int64_t bytes = N * K;
+    if (M == 1) return bytes <= int64_t(1) << 26;
+    return N <= 4096 && ((M == 2 && bytes <= int64_t(1) << 24) ||
+                         (M <= 4 && bytes <= int64_t(1) << 23));
+}
+
+// As many warps to a channel's K as keep all warps within 32 on every SM (8192
+// channels 1, 4096 channels 2, whatever K), each with at least 1024 bytes of it.
+template <typename T, int TOKENS>
+int launch_vec(const int8_t* A, const int8_t* B, int64_t lda, int64_t ldb, const I8Params& p,
+               const DeviceInfo& dev, cudaStream_t stream) {
+    int ksplit = 1;
+    while (ksplit < kI8VecWarps && p.K / (ksplit * 2) >= 1024 &&
+           ceil_div(p.N, kI8VecRows) * ksplit * 2 <= int64_t(dev.num_sms) * 32)
+        ksplit *= 2;
+    const unsigned grid = unsigned(ceil_div(p.N, kI8VecRows * (kI8VecWarps / ksplit)));
+    ridge_gemm_i8_vec<T, TOKENS><<<grid, kI8VecWarps * 32, 0, stream>>>(A, B, lda, ldb, ksplit, p);
+    return int(cudaGetLastError());
+}
+
 template <typename T>
 int launch_empty(const I8Params& p, cudaStream_t stream) {
     const dim3 grid(unsigned(ceil_div(p.N, 256)), unsigned(std::min(p.M, 65535)));
@@ -291,6 +317,15 @@ int launch_empty(const I8Params& p, cudaStream_t stream) {
 template <typename T>
 int run_product(const int8_t* A, const int8_t* B, int32_t type, int64_t lda, int64_t ldb,
                 I8Params p, const DeviceInfo& dev, cudaStream_t stream) {
+    bool vec = vec_serves(p.M, p.N, p.K);
+#ifdef RIDGE_I8_PROBE
+    if (std::getenv("RIDGE_I8_PLAN")) vec = false;
+#endif
+    if (vec) {
+        if (p.M == 1) return launch_vec<T, 1>(A, B, lda, ldb, p, dev, stream);
+        if (p.M == 2) return launch_vec<T, 2>(A, B, lda, ldb, p, dev, stream);
+        return launch_vec<T, 4>(A, B, lda, ldb, p, dev, stream);
+    }
     int pairs = 0;
     int st = resident_pairs<T>(dev, &pairs);
     if (st != RIDGE_OK) return st;

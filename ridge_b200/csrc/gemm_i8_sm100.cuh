@@ -11,20 +11,32 @@
 // of the sum or the split of K. The epilogue rounds the integer to FP32, applies
 // sb, sa and the bias there, and rounds once more to the type of C.
 //
-// Both kernels below feed one MMA thread from a ring of 128-byte-wide K blocks
+// The first two kernels below feed one MMA thread from a ring of 128-byte-wide K blocks
 // (one 128B swizzle row, 128 values of K, four K = 32 MMAs) filled by one TMA
 // thread, as the FP16 family does. They differ in which operand lies along the
 // 128 TMEM lanes:
 //
 //   ridge_gemm_i8_tile    rows of A on the lanes: 256 x BN tiles by 2-CTA pairs,
-//                         persistent, two accumulators. For work that fills the
-//                         GPU; bound by the tensor cores.
+//                         persistent, two accumulators, so that a tile's drain
+//                         hides behind the next one's MMAs. For work that fills the
+//                         GPU. Bound by the tensor cores and, in long runs, by the
+//                         power they take: 8192^3 328 us (3350 TOP/s) in a burst,
+//                         390 us back to back; 2048 x 14336 x 4096 82 us (tensor
+//                         pipe 83% of active cycles, the rest the first loads, the
+//                         last drain and the strips of the last round). A short K
+//                         leaves the drain uncovered: 8192 x 8192 x 512 50 us, 3.2
+//                         us a tile, against 22 us for its bytes.
 //   ridge_gemm_i8_stream  rows of B on the lanes, up to 256 rows of A as columns,
 //                         so few tokens waste no lanes: the MMA's cost falls with
-//                         the columns, not below 128 tokens' worth. K is split over
-//                         the CTAs of a cluster, which add their integer sums
-//                         through distributed shared memory. For few tokens; bound
-//                         by the bytes of B.
+//                         the columns. K is split over the CTAs of a cluster, which
+//                         add their integer sums through distributed shared memory:
+//                         exact in any order, no workspace, nothing to clear. For
+//                         few tokens. Bound by the bytes of B and a fixed 3.5 us of
+//                         launch, set-up, exchange and stores: 1 x 8192 x 8192 14.2
+//                         us (4.7 TB/s); with 128 tokens 18.4 us, when A passes
+//                         through every CTA as well.
+//   ridge_gemm_i8_vec     a token or a few and few enough bytes of B: no tensor
+//                         cores, no set-up.
 
 #pragma once
 
@@ -39,7 +51,7 @@
 
 namespace ridge_b200 {
 
-constexpr int kI8BK = 128;          // K per ring stage: bytes of one swizzle row
+constexpr int kI8BK = 128;          // K block: bytes of one swizzle row
 constexpr int kI8MaxStages = 12;
 constexpr int kI8BarrierBytes = 256;
 constexpr int kI8AlignSlack = 1024;
@@ -53,7 +65,7 @@ struct I8Params {
     long long ldc;
     int bn;         // tile: columns of C per tile (64, 128, 192, 256); stream: rows of A (16..256)
     int whole;      // tile: tiles computed bn wide; each later one is cut into `cut` narrower
-    int cut;        // ones (1, 2 or 4, widths of whole 64s) that fill the last round
+    int cut;        // ones (1 to 4, widths of whole 64s) that fill the last round
     int stages;
     int sub;        // stream: K blocks to a ring stage (1 or 2)
     int groupM;
@@ -723,6 +735,117 @@ __global__ void __launch_bounds__(kI8StreamThreads)
     if constexpr (SPLIT > 1) {
         __syncwarp();
         cluster_sync();  // no rank leaves while another reads its sums
+    }
+}
+
+// ------------------------------------------------------------------ one to four tokens
+
+constexpr int kI8VecWarps = 8;
+
+// 16 bytes of B, read once: not kept in L1.
+__device__ __forceinline__ int4 ld_once(const int8_t* p) {
+    int4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
+__device__ __forceinline__ int dot16(int4 a, int4 b, int sum) {
+    sum = __dp4a(a.x, b.x, sum);
+    sum = __dp4a(a.y, b.y, sum);
+    sum = __dp4a(a.z, b.z, sum);
+    return __dp4a(a.w, b.w, sum);
+}
+
+// Two channels at a time by a warp, whose lanes take 16 bytes of each in turn;
+// `ksplit` warps of a CTA share the channels' K. A comes from L1, once for both
+// channels. No set-up and no barrier stand before the first load (the streaming
+// kernel's 3.5 us), and lanes multiply four bytes an instruction: bound by the
+// bytes of B as long as a token or two share them, then by reading A again and
+// again. 1 x 4096 x 4096 5.1 us (the streaming kernel 6.9), 1 x 1000 x 1000 2.6
+// (4.3), 1 x 8192 x 8192 13.6 (13.8).
+constexpr int kI8VecRows = 2;
+
+template <typename T, int TOKENS>
+__global__ void __launch_bounds__(kI8VecWarps * 32)
+    ridge_gemm_i8_vec(const int8_t* __restrict__ A, const int8_t* __restrict__ B, long long lda,
+                      long long ldb, int ksplit, const I8Params p) {
+    __shared__ int s_sum[kI8VecWarps][kI8VecRows * TOKENS];
+    constexpr int ROWS = kI8VecRows;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = warp / ksplit, part = warp - group * ksplit;
+    const long long f0 = ((long long)blockIdx.x * (kI8VecWarps / ksplit) + group) * ROWS;
+    const int chunks = p.K / 16;
+    const int c0 = int((long long)chunks * part / ksplit);
+    const int c1 = int((long long)chunks * (part + 1) / ksplit);
+    // Channels and tokens past the end repeat the last one and are not stored.
+    const int8_t* b[ROWS];
+    const int8_t* a[TOKENS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) b[r] = B + min(f0 + r, (long long)p.N - 1) * ldb;
+#pragma unroll
+    for (int t = 0; t < TOKENS; ++t) a[t] = A + min(t, p.M - 1) * lda;
+    int sum[ROWS][TOKENS] = {};
+    constexpr int kUnroll = 4;  // 128 bytes of B in flight per lane
+    int c = c0 + lane;
+    for (; c + 32 * (kUnroll - 1) < c1; c += 32 * kUnroll) {
+        int4 vb[kUnroll][ROWS];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) vb[u][r] = ld_once(b[r] + 16ll * (c + 32 * u));
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+            for (int t = 0; t < TOKENS; ++t) {
+                const int4 va = *reinterpret_cast<const int4*>(a[t] + 16ll * (c + 32 * u));
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) sum[r][t] = dot16(va, vb[u][r], sum[r][t]);
+            }
+    }
+    for (; c < c1; c += 32)
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const int4 vb = ld_once(b[r] + 16ll * c);
+#pragma unroll
+            for (int t = 0; t < TOKENS; ++t)
+                sum[r][t] =
+                    dot16(*reinterpret_cast<const int4*>(a[t] + 16ll * c), vb, sum[r][t]);
+        }
+    // The last K % 16 bytes of a row, one to a lane: nothing past them is read.
+    if (part == 0 && lane < p.K - chunks * 16) {
+        const int k = chunks * 16 + lane;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+            for (int t = 0; t < TOKENS; ++t) sum[r][t] += int(a[t][k]) * int(b[r][k]);
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int t = 0; t < TOKENS; ++t)
+            sum[r][t] = __reduce_add_sync(0xffffffffu, sum[r][t]);
+    if (ksplit > 1) {
+        if (lane == 0)
+#pragma unroll
+            for (int i = 0; i < ROWS * TOKENS; ++i) s_sum[warp][i] = sum[i / TOKENS][i % TOKENS];
+        __syncthreads();
+        if (part != 0) return;
+        for (int w = 1; w < ksplit; ++w)
+#pragma unroll
+            for (int i = 0; i < ROWS * TOKENS; ++i)
+                sum[i / TOKENS][i % TOKENS] += s_sum[warp + w][i];
+    }
+    const T* bias = static_cast<const T*>(p.bias);
+    T* C = static_cast<T*>(p.C);
+#pragma unroll
+    for (int i = 0; i < ROWS * TOKENS; ++i) {
+        const int r = i / TOKENS, t = i % TOKENS;
+        const long long f = f0 + r;
+        if (lane == i && f < p.N && t < p.M)
+            C[t * p.ldc + f] = OutType<T>::down(fmaf(float(sum[r][t]) * p.sb[f], p.sa[t],
+                                                     bias ? OutType<T>::up(bias[f]) : 0.0f));
     }
 }
 

@@ -18,6 +18,12 @@
 //
 // and rstd never touches the elements. The other operators have v = y, rstd = 1.
 //
+// Bound by memory: 8192 x 8192 BF16 with a residual (read 2, write 1 and the 8-bit
+// rows) 72 us, 6.5 TB/s; gate and up of 4096 x 14336 FP16 52 us, 5.7 TB/s;
+// quantising 14336 x 4096 BF16 30 us, 5.8 TB/s; one row of 4096 2 us, a launch.
+// Rows that are no whole 16 bytes are read element by element (333 x 5003 FP32 8.4
+// us, 1 TB/s).
+//
 // Numerics: everything between load and store is FP32. q_j is v_j * inv + 1.5 * 2^23
 // in one fused multiply-add: the sum's unit is 1, so the add rounds the exact
 // product to the nearest whole number (ties to even) and the low byte of its

@@ -228,7 +228,8 @@ def _check_gemm(out, a, sa, b, sb, bias):
 
 
 # One token to many; around every token tile, channel tile and K block; below one of each.
-SHAPES = [(1, 1, 1), (1, 16, 16), (1, 128, 128), (1, 8192, 1024), (2, 130, 96), (7, 1000, 129),
+SHAPES = [(1, 1, 1), (1, 16, 16), (1, 9000, 8191), (2, 4095, 2049), (3, 129, 4100), (4, 4096, 2047),
+          (2, 33, 8), (4, 7, 40000), (1, 128, 128), (1, 8192, 1024), (2, 130, 96), (7, 1000, 129),
           (15, 127, 31), (16, 256, 4096), (17, 300, 640), (33, 4096, 512), (64, 129, 1000),
           (100, 640, 2048), (128, 8192, 256), (129, 1003, 385), (255, 257, 130), (256, 512, 1024),
           (257, 256, 128), (300, 1000, 2600), (517, 1003, 260), (512, 512, 4096),
@@ -257,6 +258,18 @@ def test_gemm_more_tiles_than_pairs(shape, dtype):
     a, sa, b, sb = _operands(*shape, seed=8)
     bias = _rand((shape[1],), dtype, 9)
     _check_gemm(rb.gemm_i8(a, sa, b, sb, bias=bias, dtype=dtype), a, sa, b, sb, bias)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("N,K", [(4096, 4096), (1003, 1000), (5000, 333), (16, 16384), (3, 15)])
+def test_gemm_rows_do_not_depend_on_the_batch(N, K, dtype):
+    """A token's row is the same bits whichever kernel and tile the batch around it takes."""
+    a, sa, b, sb = _operands(700, N, K, 11)
+    bias = _rand((N,), dtype, 12)
+    whole = rb.gemm_i8(a, sa, b, sb, bias=bias, dtype=dtype)
+    for M in (1, 2, 3, 4, 5, 64, 130, 256, 257):
+        part = rb.gemm_i8(a[:M], sa[:M], b, sb, bias=bias, dtype=dtype)
+        assert torch.equal(part, whole[:M]), M
 
 
 @pytest.mark.parametrize("M", [3, 200, 600])
