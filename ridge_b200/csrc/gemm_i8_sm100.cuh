@@ -20,9 +20,9 @@
 //                         persistent, two accumulators, so that a tile's drain
 //                         hides behind the next one's MMAs. For work that fills the
 //                         GPU. Bound by the tensor cores and, in long runs, by the
-//                         power they take: 8192^3 328 us (3350 TOP/s) in a burst,
-//                         390 us back to back; 2048 x 14336 x 4096 82 us (tensor
-//                         pipe 83% of active cycles, the rest the first loads, the
+//                         power they take: 8192^3 326 us (3370 TOP/s) in a burst,
+//                         384 us back to back; 2048 x 14336 x 4096 82 us (tensor
+//                         pipe 78 to 83% of active cycles, the rest the first loads, the
 //                         last drain and the strips of the last round). A short K
 //                         leaves the drain uncovered: 8192 x 8192 x 512 50 us, 3.2
 //                         us a tile, against 22 us for its bytes.
@@ -32,9 +32,10 @@
 //                         add their integer sums through distributed shared memory:
 //                         exact in any order, no workspace, nothing to clear. For
 //                         few tokens. Bound by the bytes of B and a fixed 3.5 us of
-//                         launch, set-up, exchange and stores: 1 x 8192 x 8192 14.2
-//                         us (4.7 TB/s); with 128 tokens 18.4 us, when A passes
-//                         through every CTA as well.
+//                         launch, set-up, exchange and stores: 8 x 8192 x 8192 14.6
+//                         us (4.6 TB/s), 1 x 16384 x 16384 44 us (6.1 TB/s); with
+//                         128 tokens 17.8 us, when A passes through every CTA as
+//                         well.
 //   ridge_gemm_i8_vec     a token or a few and few enough bytes of B: no tensor
 //                         cores, no set-up.
 
