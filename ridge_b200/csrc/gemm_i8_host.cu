@@ -6,8 +6,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <cstdlib>
-#include <cstdio>
 #include <cstring>
 
 #include "../../include/ridge_b200.h"
@@ -42,7 +40,8 @@ struct Plan {
     int sub;          // stream: K blocks to a stage
     int split;        // stream: CTAs of a cluster that share K
     int64_t items;    // units of work: tiles and strips, or CTAs of the streaming kernel
-    int whole, cut;   // tile: see I8Params
+    int64_t whole;    // tile: see I8Params
+    int cut;
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -64,7 +63,7 @@ Plan tile_plan(int64_t M, int64_t N, int bn, int pairs) {
     p.cut = 1;
     for (int cut = 2; last > 0 && cut <= bn / 64; ++cut)
         if (bn % (64 * cut) == 0 && last * cut <= pairs) p.cut = cut;
-    p.whole = int(p.cut > 1 ? tiles - last : tiles);
+    p.whole = p.cut > 1 ? tiles - last : tiles;
     p.items = p.whole + (tiles - p.whole) * p.cut;
     return p;
 }
@@ -151,16 +150,6 @@ double tile_time(const Plan& p, int64_t num_kb, int elem_size, int pairs) {
 // The kernel and tile with the least estimated time. Sums are exact integers, so
 // results do not depend on the choice.
 Plan make_plan(int64_t M, int64_t N, int64_t K, int elem_size, int num_sms, int pairs) {
-#ifdef RIDGE_I8_PROBE
-    if (const char* v = std::getenv("RIDGE_I8_PLAN")) {
-        int s = 0, bn = 0, stages = 0, split = 0, sub = 1;
-        std::sscanf(v, "%d,%d,%d,%d,%d", &s, &bn, &stages, &split, &sub);
-        Plan p = s ? stream_plan(M, N, K, bn, split, num_sms) : tile_plan(M, N, bn, pairs);
-        p.stages = stages;
-        p.sub = sub;
-        return p;
-    }
-#endif
     const int64_t num_kb = ceil_div(K, kI8BK);
     Plan best{};
     double best_time = 0;
@@ -265,7 +254,7 @@ int resident_pairs(const DeviceInfo& dev, int* pairs) {
 
 template <typename T, int SPLIT>
 int launch_stream(const Plan& plan, const CUtensorMap& a, const CUtensorMap& b,
-                    const I8Params& p, const DeviceInfo& dev, cudaStream_t stream) {
+                  const I8Params& p, const DeviceInfo& dev, cudaStream_t stream) {
     static std::atomic<bool> ready[kMaxDevices];
     const int st = allow_smem(reinterpret_cast<const void*>(&ridge_gemm_i8_stream<T, SPLIT>),
                               &ready[dev.device]);
@@ -317,11 +306,7 @@ int launch_empty(const I8Params& p, cudaStream_t stream) {
 template <typename T>
 int run_product(const int8_t* A, const int8_t* B, int32_t type, int64_t lda, int64_t ldb,
                 I8Params p, const DeviceInfo& dev, cudaStream_t stream) {
-    bool vec = vec_serves(p.M, p.N, p.K);
-#ifdef RIDGE_I8_PROBE
-    if (std::getenv("RIDGE_I8_PLAN")) vec = false;
-#endif
-    if (vec) {
+    if (vec_serves(p.M, p.N, p.K)) {
         if (p.M == 1) return launch_vec<T, 1>(A, B, lda, ldb, p, dev, stream);
         if (p.M == 2) return launch_vec<T, 2>(A, B, lda, ldb, p, dev, stream);
         return launch_vec<T, 4>(A, B, lda, ldb, p, dev, stream);
@@ -352,7 +337,7 @@ int run_product(const int8_t* A, const int8_t* B, int32_t type, int64_t lda, int
     // us against 340 with 8), 8 write C in a better order while it is short
     // (8192 x 8192 x 512 50 us against 54.6).
     p.groupM = p.K >= 4096 ? 16 : 8;
-    p.whole = plan.whole;
+    p.whole = int(plan.whole);
     p.cut = plan.cut;
     CUtensorMap strip = b, c;
     if (plan.cut > 1) {
