@@ -21,8 +21,7 @@
 // Bound by memory: 8192 x 8192 BF16 with a residual (read 2, write 1 and the 8-bit
 // rows) 72 us, 6.5 TB/s; gate and up of 4096 x 14336 FP16 52 us, 5.7 TB/s;
 // quantising 14336 x 4096 BF16 30 us, 5.8 TB/s; one row of 4096 2 us, a launch.
-// Rows that are no whole 16 bytes are read element by element (333 x 5003 FP32 8.4
-// us, 1 TB/s).
+// Rows that start anywhere take 1.6 to 2 times as long (below).
 //
 // Numerics: everything between load and store is FP32. q_j is v_j * inv + 1.5 * 2^23
 // in one fused multiply-add: the sum's unit is 1, so the add rounds the exact
@@ -286,7 +285,7 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) ridge_row_i8(const RowParam
     // its registers (112 against 64 a thread) would halve the rows in flight on an
     // SM, and all rows share it, so it comes from L1 or L2 when it is needed
     // (8192 x 8192 BF16 with a residual: 136 us with it early, 78 without).
-    constexpr bool kEarlyW = kW && (VEC == 1 ? CH <= 8 : CH <= 2);
+    constexpr bool kEarlyW = kW && CH <= 2;
     C cx[CH], cr[kR ? CH : 1], cw[kEarlyW ? CH : 1];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -323,100 +322,289 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) ridge_row_i8(const RowParam
     if (threadIdx.x == 0) p.scale[row] = s.scale;
 }
 
-// Rows longer than a CTA's registers hold: read twice (the second time mostly
-// from L2), reduce in the first pass and write in the second. x + r is stored
-// in the second pass only, each element by the thread that has just read it,
-// so h may be x or r here too.
-template <typename T, int OP, int VEC>
-__global__ void __launch_bounds__(1024) ridge_row_i8_long(const RowParams p) {
+// ------------------------------------------------------------------ rows that start anywhere
+//
+// A row whose start or length is no multiple of 16 bytes is cut into the same
+// windows of VEC elements (16 bytes) from its start. A window lies across two
+// aligned 16-byte words of memory, at the same offset `s` for the whole row, so
+// it is read as two loads and a shift. The sum x + r goes through shared memory,
+// where the reduction's barrier stands anyway, and is written as aligned words.
+// Only words that lie inside the row are touched as a whole; at its two ends
+// elements go one by one.
+// Against reading every element by itself, 8192 x 8191 BF16: quantise 58 us
+// (154), norm with a residual 153 (210), gate 92 (151).
+
+// 16 bytes from `s` bytes into the 32 of lo and hi.
+__device__ __forceinline__ uint4 shift_words(const uint4& lo, const uint4& hi, uint32_t s) {
+    const uint32_t b = (s & 3u) * 8u;
+    switch (s >> 2) {
+        case 0:
+            return make_uint4(__funnelshift_r(lo.x, lo.y, b), __funnelshift_r(lo.y, lo.z, b),
+                              __funnelshift_r(lo.z, lo.w, b), __funnelshift_r(lo.w, hi.x, b));
+        case 1:
+            return make_uint4(__funnelshift_r(lo.y, lo.z, b), __funnelshift_r(lo.z, lo.w, b),
+                              __funnelshift_r(lo.w, hi.x, b), __funnelshift_r(hi.x, hi.y, b));
+        case 2:
+            return make_uint4(__funnelshift_r(lo.z, lo.w, b), __funnelshift_r(lo.w, hi.x, b),
+                              __funnelshift_r(hi.x, hi.y, b), __funnelshift_r(hi.y, hi.z, b));
+        default:
+            return make_uint4(__funnelshift_r(lo.w, hi.x, b), __funnelshift_r(hi.x, hi.y, b),
+                              __funnelshift_r(hi.y, hi.z, b), __funnelshift_r(hi.z, hi.w, b));
+    }
+}
+
+template <typename T>
+using Window = Chunk<T, kVecOf<T>>;
+
+// Elements e .. e + VEC - 1 of a row of D; zeros past its end.
+template <typename T>
+__device__ __forceinline__ Window<T> load_window(const T* row, int64_t e, int64_t D) {
+    constexpr int V = kVecOf<T>;
+    union {
+        uint4 words;
+        T elems[V];
+    } u;
+    const T* at = row + e;
+    const uint32_t s = uint32_t(reinterpret_cast<uintptr_t>(at) & 15u);
+    const int before = int(s) / int(sizeof(T));  // elements between the aligned word and `at`
+    const uint4* word = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(at) - s);
+    if (s == 0 && e + V <= D) {
+        u.words = word[0];
+    } else if (e >= before && e - before + 2 * V <= D) {
+        u.words = shift_words(word[0], word[1], s);
+    } else {
+        u.words = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (e + i < D) u.elems[i] = at[i];
+    }
+    Window<T> c;
+    *reinterpret_cast<uint4*>(&c) = u.words;
+    return c;
+}
+
+// The window at e to a row of D, by all lanes of a warp whose windows follow one
+// another (the long rows' way, without shared memory).
+template <typename T>
+__device__ __forceinline__ void store_window(T* row, int64_t e, int64_t D, const Window<T>& c) {
+    constexpr int V = kVecOf<T>;
+    union {
+        uint4 words;
+        T elems[V];
+    } u;
+    u.words = *reinterpret_cast<const uint4*>(&c);
+    uint4 next;  // the next lane's window
+    next.x = __shfl_down_sync(0xffffffffu, u.words.x, 1);
+    next.y = __shfl_down_sync(0xffffffffu, u.words.y, 1);
+    next.z = __shfl_down_sync(0xffffffffu, u.words.z, 1);
+    next.w = __shfl_down_sync(0xffffffffu, u.words.w, 1);
+    T* at = row + e;
+    const int lane = threadIdx.x & 31;
+    // Bytes and elements from the window's start to the next 16-byte boundary.
+    const uint32_t off = uint32_t(16 - (reinterpret_cast<uintptr_t>(at) & 15u)) & 15u;
+    const int head = int(off) / int(sizeof(T));
+    // From the boundary on: one store with the next lane's first elements, which
+    // that lane then leaves out.
+    const bool joined = e + head + V <= D && (lane < 31 || off == 0);
+    if (joined) *reinterpret_cast<uint4*>(at + head) = shift_words(u.words, next, off);
+    const bool keep_head = lane == 0 || e + head > D;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (e + i < D && (i < head ? keep_head : !joined)) at[i] = u.elems[i];
+}
+
+// The 8-bit values of a window.
+template <int V>
+__device__ __forceinline__ void store_q_window(int8_t* row, int64_t e, int64_t D,
+                                               const float (&v)[V], float inv, bool zero) {
+    if (e + V <= D) {
+        store_q<V>(row + e, v, inv, zero);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (e + i < D) row[e + i] = zero ? int8_t(0) : int8_t(round_bits(v[i], inv) & 0xffu);
+    }
+}
+
+// ridge_row_i8 for such rows; q itself starts on VEC bytes.
+template <typename T, int OP, int CH, int MAXT>
+__global__ void __launch_bounds__(MAXT) ridge_row_i8_odd(const RowParams p) {
     constexpr bool kR = OP == kNormAdd || OP == kSiluMul;
     constexpr bool kW = OP == kNorm || OP == kNormAdd;
-    const int64_t row = blockIdx.x;
+    constexpr int V = kVecOf<T>;
+    const int64_t row = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
+    if (row >= p.M) return;
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
     const T* r = static_cast<const T*>(p.r) + (kR ? row * p.ldr : 0);
     const T* w = static_cast<const T*>(p.w);
-    using C = Chunk<T, VEC>;
-    const int64_t step = int64_t(blockDim.x) * VEC;
+    // kNormAdd: the row of sums as it will be stored, and one word that is read past it.
+    extern __shared__ uint4 s_rows[];
+    uint4* s_row = s_rows + threadIdx.y * (CH * blockDim.x + 1);
+    Window<T> cx[CH], cr[kR ? CH : 1];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int e = (c * int(blockDim.x) + int(threadIdx.x)) * V;
+        cx[c] = load_window(x, e, p.D);
+        if constexpr (kR) cr[c] = load_window(r, e, p.D);
+    }
+    float v[CH][V];
     float sumsq = 0.0f;
     float top = 0.0f;
-    C cx, cr, cw, h;
-    float v[VEC];
-    auto load = [&](int64_t e) {
-        cx = *reinterpret_cast<const C*>(x + e);
-        if constexpr (kR) cr = *reinterpret_cast<const C*>(r + e);
-        if constexpr (kW) cw = *reinterpret_cast<const C*>(w + e);
-    };
-    for (int64_t e = int64_t(threadIdx.x) * VEC; e < p.D; e += step) {
-        load(e);
-        take_chunk<T, OP, VEC>(cx, cr, cw, h, v, sumsq, top);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int e = (c * int(blockDim.x) + int(threadIdx.x)) * V;
+        Window<T> h, gain = cx[c];
+        if constexpr (kW) gain = load_window(w, e, p.D);
+        take_chunk<T, OP, V>(cx[c], cr[kR ? c : 0], gain, h, v[c], sumsq, top);
+        if constexpr (OP == kNormAdd)
+            s_row[c * int(blockDim.x) + int(threadIdx.x)] = *reinterpret_cast<const uint4*>(&h);
     }
     reduce_row(sumsq, top, kW);
+    if constexpr (OP == kNormAdd) {
+        __syncwarp();  // a row of one warp passes no barrier in reduce_row
+        T* out = static_cast<T*>(p.h) + row * p.ldh;
+        const T* sums = reinterpret_cast<const T*>(s_row);
+        // Elements, and bytes, before the row's first 16-byte boundary.
+        const uint32_t off = uint32_t(16 - (reinterpret_cast<uintptr_t>(out) & 15u)) & 15u;
+        const int head = int(off) / int(sizeof(T));
+        if (int(threadIdx.x) < min(head, p.D)) out[threadIdx.x] = sums[threadIdx.x];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int i = c * int(blockDim.x) + int(threadIdx.x), e = head + i * V;
+            if (e + V <= p.D)
+                *reinterpret_cast<uint4*>(out + e) = shift_words(s_row[i], s_row[i + 1], off);
+            else
+                for (int k = e; k < p.D; ++k) out[k] = sums[k];
+        }
+    }
     const RowScale s = row_scale<OP>(sumsq, top, p.D, p.eps);
     int8_t* q = p.q + row * p.ldq;
-    float unused_sum = 0.0f;
-    float unused_top = 0.0f;
-    for (int64_t e = int64_t(threadIdx.x) * VEC; e < p.D; e += step) {
-        load(e);
-        take_chunk<T, OP, VEC>(cx, cr, cw, h, v, unused_sum, unused_top);
-        if constexpr (OP == kNormAdd)
-            *reinterpret_cast<C*>(static_cast<T*>(p.h) + row * p.ldh + e) = h;
-        prescale(s, v);
-        store_q<VEC>(q + e, v, s.inv, s.zero);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int e = (c * int(blockDim.x) + int(threadIdx.x)) * V;
+        prescale(s, v[c]);
+        store_q_window(q, e, p.D, v[c], s.inv, s.zero);
     }
     if (threadIdx.x == 0) p.scale[row] = s.scale;
 }
 
-template <typename T, int OP, int VEC, int CH, int MAXT>
-cudaError_t launch_rows(const RowParams& p, int threads, int rows_per_cta, cudaStream_t stream) {
-    const dim3 block(static_cast<unsigned>(threads), static_cast<unsigned>(rows_per_cta));
-    const unsigned grid = unsigned((int64_t(p.M) + rows_per_cta - 1) / rows_per_cta);
-    ridge_row_i8<T, OP, VEC, CH, MAXT><<<grid, block, 0, stream>>>(p);
-    return cudaGetLastError();
-}
-
-// The launch shape of a row of `chunks` loads. Rows of up to 128 loads take one
-// warp, four rows to a CTA (no barrier). Longer rows take a CTA with as few
-// chunks per thread as fit when there are fewer rows than SMs -- one row's
-// latency is then all that counts -- and four per thread otherwise, so that
-// several CTAs share an SM and one row's reduction hides behind another's loads.
-template <typename T, int OP, int VEC>
-cudaError_t run_rows(const RowParams& p, int num_sms, cudaStream_t stream) {
-    const int64_t chunks = (int64_t(p.D) + VEC - 1) / VEC;
-    auto threads_for = [&](int per) { return int(((chunks + per - 1) / per + 31) / 32 * 32); };
-    if constexpr (VEC > 1) {
-        if (chunks <= 32) return launch_rows<T, OP, VEC, 1, 1024>(p, 32, 4, stream);
-        if (chunks <= 64) return launch_rows<T, OP, VEC, 2, 1024>(p, 32, 4, stream);
-        if (chunks <= 128) return launch_rows<T, OP, VEC, 4, 512>(p, 32, 4, stream);
-        if (p.M <= num_sms) {
-            if (chunks <= 1024) return launch_rows<T, OP, VEC, 1, 1024>(p, threads_for(1), 1, stream);
-            if (chunks <= 2048) return launch_rows<T, OP, VEC, 2, 1024>(p, threads_for(2), 1, stream);
+// Rows longer than a CTA's registers hold: read twice (the second time mostly
+// from L2), reduce in the first pass and write in the second. x + r is stored
+// in the second pass only. With windows (kWindows) that start anywhere; without,
+// element by element, for a q that does not start on VEC bytes.
+//
+// h may be x or r here too: each element is read in the second pass by the warp
+// that stores it, and a warp stores its windows after it has read them. (Its two
+// outer words may be read by a neighbouring warp as well, whose elements beside
+// the boundary are its own alone: what it takes from such a word it stores itself.)
+template <typename T, int OP, bool kWindows>
+__global__ void __launch_bounds__(1024) ridge_row_i8_long(const RowParams p) {
+    constexpr bool kR = OP == kNormAdd || OP == kSiluMul;
+    constexpr bool kW = OP == kNorm || OP == kNormAdd;
+    constexpr int V = kWindows ? kVecOf<T> : 1;
+    const int64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+    const T* r = static_cast<const T*>(p.r) + (kR ? row * p.ldr : 0);
+    const T* w = static_cast<const T*>(p.w);
+    T* h_row = static_cast<T*>(p.h) + (OP == kNormAdd ? row * p.ldh : 0);
+    using C = Chunk<T, V>;
+    const int64_t step = int64_t(blockDim.x) * V;
+    float sumsq = 0.0f;
+    float top = 0.0f;
+    C cx, cr, cw, h;
+    float v[V];
+    auto load = [&](const T* from, int64_t e) -> C {
+        if constexpr (kWindows) return load_window(from, e, p.D);
+        C c{};
+        if (e < p.D) c.raw[0] = *reinterpret_cast<const typename C::Raw*>(from + e);
+        return c;
+    };
+    auto take = [&](int64_t e, float& sum, float& max) {
+        cx = load(x, e);
+        if constexpr (kR) cr = load(r, e);
+        if constexpr (kW) cw = load(w, e);
+        take_chunk<T, OP, V>(cx, cr, cw, h, v, sum, max);
+    };
+    // Whole warps take part to the end of the row (first element of the warp's windows).
+    const int64_t mine = int64_t(threadIdx.x) * V, first = int64_t(threadIdx.x & ~31u) * V;
+    for (int64_t e = 0; first + e < p.D; e += step) take(mine + e, sumsq, top);
+    reduce_row(sumsq, top, kW);
+    const RowScale s = row_scale<OP>(sumsq, top, p.D, p.eps);
+    int8_t* q = p.q + row * p.ldq;
+    float unused_sum = 0.0f, unused_top = 0.0f;
+    for (int64_t i = 0; first + i < p.D; i += step) {
+        const int64_t e = mine + i;
+        take(e, unused_sum, unused_top);
+        prescale(s, v);
+        if constexpr (kWindows) {
+            if constexpr (OP == kNormAdd) store_window(h_row, e, p.D, h);
+            store_q_window(q, e, p.D, v, s.inv, s.zero);
+        } else if (e < p.D) {
+            if constexpr (OP == kNormAdd) *reinterpret_cast<C*>(h_row + e) = h;
+            store_q<V>(q + e, v, s.inv, s.zero);
         }
-        if (chunks <= 2048) return launch_rows<T, OP, VEC, 4, 512>(p, threads_for(4), 1, stream);
-        if (chunks <= 4096) return launch_rows<T, OP, VEC, 4, 1024>(p, threads_for(4), 1, stream);
-    } else {
-        if (chunks <= 128) return launch_rows<T, OP, VEC, 4, 1024>(p, 32, 4, stream);
-        if (chunks <= 4096) return launch_rows<T, OP, VEC, 4, 1024>(p, threads_for(4), 1, stream);
-        if (p.M <= num_sms && chunks <= 8192)
-            return launch_rows<T, OP, VEC, 8, 1024>(p, threads_for(8), 1, stream);
-        if (chunks <= 16384) return launch_rows<T, OP, VEC, 16, 1024>(p, threads_for(16), 1, stream);
     }
-    ridge_row_i8_long<T, OP, VEC><<<unsigned(p.M), 1024, 0, stream>>>(p);
+    if (threadIdx.x == 0) p.scale[row] = s.scale;
+}
+
+// The launch shape of a row of `chunks` 16-byte chunks. Rows of up to 128 chunks
+// take one warp, four rows to a CTA (no barrier). Longer rows take a CTA with as few
+// chunks per thread as fit when there are fewer rows than SMs -- one row's
+// latency is then all that counts -- and four per thread otherwise (two for rows
+// that start anywhere, whose windows take two loads each), so that several CTAs
+// share an SM and one row's reduction hides behind another's loads.
+template <typename T, int OP>
+cudaError_t run_rows(const RowParams& p, bool aligned, int num_sms, cudaStream_t stream) {
+    constexpr int V = kVecOf<T>;
+    const int64_t chunks = (int64_t(p.D) + V - 1) / V;
+    auto launch = [&](void (*kernel)(RowParams), int per, int rows_per_cta) {
+        const int threads = chunks <= 128 ? 32 : int(((chunks + per - 1) / per + 31) / 32 * 32);
+        const dim3 block(static_cast<unsigned>(threads), static_cast<unsigned>(rows_per_cta));
+        const unsigned grid = unsigned((int64_t(p.M) + rows_per_cta - 1) / rows_per_cta);
+        const size_t smem =
+            !aligned && OP == kNormAdd ? size_t(per * threads + 1) * rows_per_cta * 16 : 0;
+        kernel<<<grid, block, smem, stream>>>(p);
+        return cudaGetLastError();
+    };
+    const bool few = p.M <= num_sms;
+    if (aligned) {
+        if (chunks <= 32) return launch(ridge_row_i8<T, OP, V, 1, 1024>, 1, 4);
+        if (chunks <= 64) return launch(ridge_row_i8<T, OP, V, 2, 1024>, 2, 4);
+        if (chunks <= 128) return launch(ridge_row_i8<T, OP, V, 4, 512>, 4, 4);
+        if (few && chunks <= 1024) return launch(ridge_row_i8<T, OP, V, 1, 1024>, 1, 1);
+        if (few && chunks <= 2048) return launch(ridge_row_i8<T, OP, V, 2, 1024>, 2, 1);
+        if (chunks <= 2048) return launch(ridge_row_i8<T, OP, V, 4, 512>, 4, 1);
+        if (chunks <= 4096) return launch(ridge_row_i8<T, OP, V, 4, 1024>, 4, 1);
+    } else {
+        if (chunks <= 32) return launch(ridge_row_i8_odd<T, OP, 1, 1024>, 1, 4);
+        if (chunks <= 64) return launch(ridge_row_i8_odd<T, OP, 2, 512>, 2, 4);
+        if (chunks <= 128) return launch(ridge_row_i8_odd<T, OP, 4, 128>, 4, 4);
+        if (few && chunks <= 1024) return launch(ridge_row_i8_odd<T, OP, 1, 1024>, 1, 1);
+        if (chunks <= 1024) return launch(ridge_row_i8_odd<T, OP, 2, 512>, 2, 1);
+        if (chunks <= 2048) return launch(ridge_row_i8_odd<T, OP, 2, 1024>, 2, 1);
+    }
+    ridge_row_i8_long<T, OP, true><<<unsigned(p.M), 1024, 0, stream>>>(p);
     return cudaGetLastError();
 }
 
-// 16-byte loads need every row of every operand to start on 16 bytes and D to be
-// whole chunks; q then takes 8- or 4-byte stores.
+// Rows are read by plain 16-byte chunks when every row of every operand starts on
+// 16 bytes and D is whole chunks, by windows otherwise. Either way q takes stores of
+// VEC bytes; one that does not start on them is written byte by byte.
 template <typename T, int OP>
 cudaError_t run_op(const RowParams& p, int num_sms, cudaStream_t stream) {
     constexpr int V = kVecOf<T>;
     auto fits = [](const void* ptr, int64_t ld, int size, int bytes) {
         return (reinterpret_cast<uintptr_t>(ptr) % bytes) == 0 && (ld * size) % bytes == 0;
     };
-    bool vec = p.D % V == 0 && fits(p.x, p.ldx, sizeof(T), 16) && fits(p.q, p.ldq, 1, V);
-    if (OP == kNormAdd || OP == kSiluMul) vec = vec && fits(p.r, p.ldr, sizeof(T), 16);
-    if (OP == kNorm || OP == kNormAdd) vec = vec && fits(p.w, 0, 1, 16);
-    if (OP == kNormAdd) vec = vec && fits(p.h, p.ldh, sizeof(T), 16);
-    return vec ? run_rows<T, OP, V>(p, num_sms, stream) : run_rows<T, OP, 1>(p, num_sms, stream);
+    if (!fits(p.q, p.ldq, 1, V)) {
+        ridge_row_i8_long<T, OP, false><<<unsigned(p.M), 1024, 0, stream>>>(p);
+        return cudaGetLastError();
+    }
+    bool aligned = p.D % V == 0 && fits(p.x, p.ldx, sizeof(T), 16);
+    if (OP == kNormAdd || OP == kSiluMul) aligned = aligned && fits(p.r, p.ldr, sizeof(T), 16);
+    if (OP == kNorm || OP == kNormAdd) aligned = aligned && fits(p.w, 0, 1, 16);
+    if (OP == kNormAdd) aligned = aligned && fits(p.h, p.ldh, sizeof(T), 16);
+    return run_rows<T, OP>(p, aligned, num_sms, stream);
 }
 
 template <typename T>

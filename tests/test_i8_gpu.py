@@ -187,10 +187,54 @@ def test_outputs_of_the_callers_own():
             assert (buf[rest] == 77).all()
 
 
-@pytest.mark.parametrize("D", [512, 4096, 5001, 40000])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("D", [1, 7, 9, 16, 250, 1001, 2048, 4099, 9000, 16390, 40003])
+def test_rows_that_start_anywhere(D, dtype):
+    """Every offset of a row's start in 16 bytes, on every operand, each its own; what lies
+    around the rows is not written."""
+    M = 5
+    pitch = D + 11
+    for k in range(0, 9):
+        def place(t, first):
+            buf = torch.full((M * pitch + 64,), 3.0, dtype=t.dtype, device="cuda")
+            view = buf[first:].as_strided((M, D), (pitch, 1), first)
+            view.copy_(t)
+            return buf, view
+        x0, r0 = _rand((M, D), dtype, k), _rand((M, D), dtype, k + 50)
+        xb, x = place(x0, k)
+        rb_, r = place(r0, (3 * k + 1) % 9)
+        hb, h = place(torch.zeros_like(x0), (5 * k + 2) % 9)
+        wb = torch.full((D + 20,), 3.0, dtype=dtype, device="cuda")
+        w = wb[(7 * k) % 9:][:D]
+        w.copy_(_rand((D,), dtype, 7, 0.2) + 1)
+        q, s, got = rb.rms_norm_i8(x, w, residual=r, residual_out=h)
+        h64, y = _norm64(x0, r0, w, 1e-6)
+        _check_rows(q, s, y, 2 * U, _norm_tol(D))
+        half = torch.finfo(dtype).eps / 2
+        assert ((h.double() - h64).abs() <= h64.abs() * (half * 1.01 + U) + 2.0 ** -25).all()
+        h.fill_(3.0)
+        assert (hb == 3.0).all()
+        q, s = rb.quantize_i8(x)
+        _check_rows(q, s, x0.double(), 0.0, U * 1.01)
+        q, s = rb.silu_mul_i8(x, r)
+        g = x0.double()
+        e = (2 + 1.173 * g.abs().max().item() + 2) * 2 * U + 3 * U
+        _check_rows(q, s, g / (1 + torch.exp(-g)) * r0.double(), e, e + 2 * U)
+        ob, o = place(torch.zeros_like(x0), (2 * k + 3) % 9)
+        rb.dequantize_i8(q, s, out=o)
+        want = q.double() * s.double()[:, None]
+        assert ((o.double() - want).abs() <= want.abs() * (half * 1.01 + U) + 2.0 ** -25).all()
+        o.fill_(3.0)
+        assert (ob == 3.0).all()
+
+
+@pytest.mark.parametrize("D", [512, 4096, 5001, 16001, 40000, 40007])
 @pytest.mark.parametrize("into", ["residual", "x"])
 def test_norm_adds_in_place(D, into):
     x, r = _rand((33, D), torch.bfloat16, 1), _rand((33, D), torch.bfloat16, 2)
+    if D % 8:
+        x = _rand((33, D + 3), torch.bfloat16, 1)[:, 1:D + 1].clone(
+            memory_format=torch.preserve_format)
     w = _rand((D,), torch.bfloat16, 3)
     q, s, h = rb.rms_norm_i8(x, w, residual=r)
     x2, r2 = x.clone(), r.clone()
