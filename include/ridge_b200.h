@@ -289,7 +289,8 @@ int ridge_rms_norm_i8(const void* x, const void* residual, const void* weight, i
 /*
  * Gated activation with an 8-bit output: y = up * gate / (1 + exp(-gate)), then
  * as ridge_quantize_i8. gate and up are of `type`; they may be column windows of
- * one wider array.
+ * one wider array. FP32 throughout: for gate below about -87, where gate / (1 +
+ * exp(-gate)) is under 1e-36, the quotient may be 0.
  */
 int ridge_silu_mul_i8(const void* gate, const void* up, int32_t type, int8_t* q, float* scale,
                       int64_t M, int64_t D, int64_t ldg, int64_t ldu, int64_t ldq, void* stream);

@@ -167,8 +167,9 @@ __device__ __forceinline__ float max_abs(float a, float b, float c) {
 
 // x / (1 + e^-x), with one ex2 and one reciprocal of the hardware's (each within
 // 2^-22.5 relative; the exponent's rounding adds |x| 2^-23.4 to e^-x, which reaches
-// the result times e^-x / (1 + e^-x)). e^-x = inf gives -0 for finite x, and NaN
-// for x = -inf, as the formula does.
+// the result times e^-x / (1 + e^-x)). Where 1 + e^-x passes 2^126 the reciprocal
+// and the result, under 1e-36, are flushed to 0; x = -inf gives NaN, as the formula
+// does.
 __device__ __forceinline__ float silu(float x) {
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
