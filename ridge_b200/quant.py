@@ -66,6 +66,8 @@ def _rows(t, what):
 
 def _like(t, what, device, dtype, shape):
     """Checks a tensor that has to match another in device, type and shape."""
+    if t.dtype is dtype and t.shape == shape and t.device == device:
+        return
     if t.device != device:
         raise ValueError("%s is on %s, expected %s" % (what, t.device, device))
     if t.dtype != dtype:
@@ -74,8 +76,19 @@ def _like(t, what, device, dtype, shape):
         raise ValueError("%s has shape %s, expected %s" % (what, tuple(t.shape), tuple(shape)))
 
 
+def _like_rows(t, what, device, dtype, shape):
+    """The pitch of rows that have to match others in device, type and shape."""
+    if t.dtype is not dtype or t.shape != shape or t.device != device:
+        _like(t, what, device, dtype, shape)
+    pitch, step = t.stride()
+    if step == 1 and pitch >= shape[1]:
+        return pitch
+    return _rows(t, what)[2]
+
+
 def _vector(t, what, device, dtype, n):
-    _like(t, what, device, dtype, (n,))
+    if t.dtype is not dtype or t.shape != (n,) or t.device != device:
+        _like(t, what, device, dtype, (n,))
     if n > 1 and t.stride(0) != 1:
         raise ValueError("%s must be contiguous" % what)
 
@@ -103,24 +116,22 @@ def _new(shape, strides, dtype, device):
 
 
 def _given(M, D, device, out, scale):
-    """Checks the arrays that a caller passed for (q, scale)."""
+    """Checks the arrays that a caller passed for (q, scale); q's pitch."""
+    pitch = (D + 15) // 16 * 16
     if out is not None:
-        _like(out, "out", device, torch.int8, (M, D))
-        _rows(out, "out")
+        pitch = _like_rows(out, "out", device, torch.int8, (M, D))
     if scale is not None:
         _vector(scale, "scale", device, torch.float32, M)
+    return pitch
 
 
-def _outputs(M, D, device, out, scale):
-    """(q, q's pitch, scale): the given arrays or new ones."""
+def _outputs(M, D, pitch, device, out, scale):
+    """(q, scale): the given arrays or new ones."""
     if out is None:
-        pitch = (D + 15) // 16 * 16
         out = _new((M, D), (pitch, 1), torch.int8, device)
-    else:
-        pitch = max(out.stride(0), D)
     if scale is None:
         scale = _new((M,), (1,), torch.float32, device)
-    return out, pitch, scale
+    return out, scale
 
 
 def quantize_i8(x, out=None, scale=None, stream=None):
@@ -131,10 +142,10 @@ def quantize_i8(x, out=None, scale=None, stream=None):
     code = _type_code(x.dtype, "x")
     M, D, ldx = _rows(x, "x")
     device = x.device
-    _given(M, D, device, out, scale)
+    ldq = _given(M, D, device, out, scale)
 
     def call(handle):
-        q, ldq, s = _outputs(M, D, device, out, scale)
+        q, s = _outputs(M, D, ldq, device, out, scale)
         st = lib.ridge_quantize_i8(x.data_ptr(), code, q.data_ptr(), s.data_ptr(), M, D, ldx, ldq,
                                    handle)
         if st:
@@ -160,19 +171,17 @@ def rms_norm_i8(x, weight, residual=None, eps=1e-6, out=None, scale=None, residu
         raise ValueError("eps is finite and above 0, got %r" % eps)
     ldr = ldh = D
     if residual is not None:
-        _like(residual, "residual", device, dtype, x.shape)
-        ldr = _rows(residual, "residual")[2]
+        ldr = _like_rows(residual, "residual", device, dtype, (M, D))
         if residual_out is not None:
-            _like(residual_out, "residual_out", device, dtype, x.shape)
-            ldh = _rows(residual_out, "residual_out")[2]
+            ldh = _like_rows(residual_out, "residual_out", device, dtype, (M, D))
     elif residual_out is not None:
         raise ValueError("residual_out needs a residual")
-    _given(M, D, device, out, scale)
+    ldq = _given(M, D, device, out, scale)
     # An empty tensor's address is null, which at the C ABI means "not given".
     add = residual is not None and M > 0 and D > 0
 
     def call(handle):
-        q, ldq, s = _outputs(M, D, device, out, scale)
+        q, s = _outputs(M, D, ldq, device, out, scale)
         h = residual_out
         if h is None and residual is not None:
             h = _new((M, D), (D, 1), dtype, device)
@@ -192,12 +201,11 @@ def silu_mul_i8(gate, up, out=None, scale=None, stream=None):
     code = _type_code(gate.dtype, "gate")
     M, D, ldg = _rows(gate, "gate")
     device = gate.device
-    _like(up, "up", device, gate.dtype, gate.shape)
-    ldu = _rows(up, "up")[2]
-    _given(M, D, device, out, scale)
+    ldu = _like_rows(up, "up", device, gate.dtype, (M, D))
+    ldq = _given(M, D, device, out, scale)
 
     def call(handle):
-        q, ldq, s = _outputs(M, D, device, out, scale)
+        q, s = _outputs(M, D, ldq, device, out, scale)
         st = lib.ridge_silu_mul_i8(gate.data_ptr(), up.data_ptr(), code, q.data_ptr(),
                                    s.data_ptr(), M, D, ldg, ldu, ldq, handle)
         if st:
@@ -221,8 +229,7 @@ def dequantize_i8(q, scale, out=None, dtype=None, stream=None):
     device = q.device
     ldo = D
     if out is not None:
-        _like(out, "out", device, dtype, q.shape)
-        ldo = _rows(out, "out")[2]
+        ldo = _like_rows(out, "out", device, dtype, (M, D))
 
     def call(handle):
         o = _new((M, D), (D, 1), dtype, device) if out is None else out
@@ -262,8 +269,7 @@ def gemm_i8(a, a_scale, b, b_scale, bias=None, out=None, dtype=None, stream=None
         _vector(bias, "bias", device, dtype, N)
     ldc = N
     if out is not None:
-        _like(out, "out", device, dtype, (M, N))
-        ldc = _rows(out, "out")[2]
+        ldc = _like_rows(out, "out", device, dtype, (M, N))
 
     def call(handle):
         o = _new((M, N), (N, 1), dtype, device) if out is None else out
