@@ -59,14 +59,15 @@ int run(int op, int32_t type, RowParams p, int64_t M, int64_t D, void* stream_v)
 
 // Values of 8-bit rows: out = scale[row] * q, one rounding to T. A thread takes
 // 16 values (one 16-byte load, 32 or 64 bytes of stores) at a time; blockDim.x
-// threads walk a row and blockDim.y rows share a CTA, so short rows fill one.
-// 8192 x 8192 to BF16 33 us, 6.1 TB/s.
+// threads walk a row and blockDim.y rows share a CTA, so short rows fill one. The
+// last rows go first: behind a quantising kernel they are the ones still in L2
+// (14336 x 4096 BF16, both ways 63.8 -> 62.6 us). 8192 x 8192 to BF16 33 us, 6.1 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(256)
     ridge_dequantize_i8(const int8_t* __restrict__ q, const float* __restrict__ scale,
                         T* __restrict__ out, int M, int D, int64_t ldq, int64_t ldo) {
-    const int64_t row = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
-    if (row >= M) return;
+    const int64_t row = int64_t(M) - 1 - (int64_t(blockIdx.x) * blockDim.y + threadIdx.y);
+    if (row < 0) return;
     const float s = scale[row];
     const int8_t* src = q + row * ldq;
     T* dst = out + row * ldo;
@@ -116,8 +117,8 @@ __global__ void __launch_bounds__(256)
     ridge_dequantize_i8_odd(const int8_t* __restrict__ q, const float* __restrict__ scale,
                             T* __restrict__ out, int M, int D, int64_t ldq, int64_t ldo) {
     constexpr int V = kVecOf<T>;
-    const int64_t row = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
-    if (row >= M) return;
+    const int64_t row = int64_t(M) - 1 - (int64_t(blockIdx.x) * blockDim.y + threadIdx.y);
+    if (row < 0) return;
     const float s = scale[row];
     const int8_t* src = q + row * ldq;
     T* dst = out + row * ldo;
